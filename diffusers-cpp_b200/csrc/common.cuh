@@ -26,6 +26,9 @@ enum DeviceError : int {
   kDevTimeoutAttn = 7,      // attention pipeline wait timed out
   kDevTimeoutPeer = 8,      // tensor-parallel barrier: a peer GPU did not arrive
   kDevBadIndex = 9,         // an embedding id outside the table
+  kDevBadCache = 10,        // a length, block id or slot outside the paged cache
+  kDevNoBlocks = 11,        // a step plan that needs more free blocks or token rows than there are
+  kDevTimeoutKv = 12,       // paged attention pipeline wait timed out
 };
 
 constexpr unsigned long long kWaitTimeoutNs = 1000ull * 1000ull * 1000ull;  // 1 s

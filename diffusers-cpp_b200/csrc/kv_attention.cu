@@ -1,0 +1,572 @@
+// Attention of a batch's new tokens over the paged key / value cache.
+//
+//   o[t, h] = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),  s_j = scale q[t, h] . k_j,
+// j over the request's cached keys (causal: up to the token's own position); a row
+// without a key is 0.  Sums, maxima and the scores are f32; the numerators are
+// rounded once to the cache's type (half a step: 2^-9 of each, as the output's own
+// rounding) because the matrix instructions take their operands in it.
+//
+// Rows of one key / value head: the `group` query heads that share it times the
+// tokens of a unit, so that K and V are read once for all of them.
+#include "kv_sched.cuh"
+
+#include <algorithm>
+#include <atomic>
+
+namespace dcpp {
+
+namespace {
+
+__device__ __forceinline__ float kv_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <bool F16>
+__device__ __forceinline__ uint32_t kv_pack2(float lo, float hi) {
+  if constexpr (F16) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    return pack_bf16x2(lo, hi);
+  }
+}
+
+// Bounded wait that looks at nothing but its barrier and the clock: another
+// kernel's recorded error does not end this one's work.
+__device__ __forceinline__ bool kv_wait(uint64_t* bar, uint32_t parity, int* err) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const unsigned long long t0 = globaltimer();
+  for (;;) {
+    if (mbar_try_wait_sleep(bar, parity, 20000u)) return true;
+    if (globaltimer() - t0 > kWaitTimeoutNs) {
+      record_error(err, kDevTimeoutKv);
+      return false;
+    }
+  }
+}
+
+__device__ __forceinline__ void named_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+template <bool F16>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (F16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// ------------------------------------------------------------ few query rows
+// Up to 32 rows per unit (single tokens, a few drafted ones): bound by reading K
+// and V once from HBM, so the tensor work only has to stay out of the way:
+// mma.sync m16n8k16 on 16 or 32 rows.  Two CTAs per SM, each with a ring of 3
+// stages of 64 keys (K 16 KB + V 16 KB, two 128-byte-swizzled halves of the head
+// dimension each) that one warp fills with TMA, a box for each piece of a block.
+// The four consumer warps each own 16 keys of every tile: scores, running maximum,
+// numerators and all 128 output columns of their keys, so the loop has no barrier
+// among them; their four partial results are joined once per unit.
+constexpr int kRKT = 64;
+constexpr int kRStages = 3;
+constexpr int kRHalf = kRKT * 128;          // 8 KB: 64 keys x 64 channels
+constexpr int kRStageBytes = 4 * kRHalf;    // K lo, K hi, V lo, V hi
+constexpr int kRThreads = 160;              // 4 consumer warps + the producer
+constexpr int kRJoinBytes = 8192;           // Q rows, later the partial sums being joined
+constexpr int kRSmem = kRStages * kRStageBytes + kRJoinBytes + 1024;
+constexpr int kRMinTiles = 2;
+
+template <int MT, bool F16>
+__global__ void __launch_bounds__(kRThreads, 2)
+    kv_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                   const __grid_constant__ KvAttnArgs p) {
+  constexpr int R = 16 * MT;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* join = smem + kRStages * kRStageBytes;
+  __shared__ uint64_t full[kRStages], empty[kRStages];
+  __shared__ float2 s_ml[4][R];
+  __shared__ KvSchedSmem<kRThreads> sched;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < kRStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 4);
+    }
+    fence_barrier_init();
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  KvRange range;
+  KvPos at;
+  const bool have = kv_locate<kRKT, kRThreads, kRMinTiles>(p, sched, range, at, [&](const KvRange& r) {
+    return static_cast<int>(blockIdx.x) < r.parts ? kv_cut(r, blockIdx.x) : static_cast<int64_t>(-1);
+  });
+  __syncthreads();  // barriers initialised
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (!have) return;
+  int64_t left = kv_cut(range, blockIdx.x + 1) - kv_cut(range, blockIdx.x);
+
+  if (warp == 4) {
+    // Producer: lane -> (K or V, half, box); the block ids come from the table 32 at
+    // a time, the next 32 fetched ahead.
+    const int boxes = kRKT / p.box_rows;             // 1, 2 or 4 boxes per tile and half
+    const int box = lane & (boxes - 1);
+    const int part = lane / boxes;                   // 0, 1: K halves; 2, 3: V halves; more: idle
+    const int bs_mask = (1 << p.block_shift) - 1;
+    int it = 0;
+    bool ok = true;
+    while (left > 0 && ok) {
+      const int n = static_cast<int>(min(left, static_cast<int64_t>(at.n_tiles - at.tile)));
+      const int32_t* row = p.table + at.b * p.max_blocks;
+      const int n_ids = (at.s.kv + bs_mask) >> p.block_shift;
+      int win = (at.tile * kRKT) >> p.block_shift;   // first block id held
+      auto fetch = [&](int i) { return i < n_ids ? __ldg(row + i) : -1; };
+      int cur = fetch(win + lane), nxt = fetch(win + 32 + lane);
+      for (int j = at.tile; j < at.tile + n && ok; ++j, ++it) {
+        const int key0 = j * kRKT + box * p.box_rows;
+        int idx = key0 >> p.block_shift;
+        if (__shfl_sync(0xffffffffu, idx, 0) - win >= 32) {  // a tile's boxes never straddle a window
+          win += 32;
+          cur = nxt;
+          nxt = fetch(win + 32 + lane);
+        }
+        const int blk = __shfl_sync(0xffffffffu, cur, idx - win);
+        const bool load = part < 4 && key0 < at.s.kv;
+        if (load && (blk < 0 || blk >= p.n_blocks)) record_error(p.err, kDevBadCache);
+        const int c3 = blk < 0 || blk >= p.n_blocks ? p.n_blocks : blk;  // one past the end: TMA fills zeros
+        const int st = it % kRStages;
+        ok = kv_wait(&empty[st], ((it / kRStages) & 1) ^ 1, p.err);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const int loads = __popc(__ballot_sync(0xffffffffu, load));
+        if (lane == 0) mbar_arrive_expect_tx(&full[st], loads * p.box_rows * 128);
+        __syncwarp();
+        if (load) {
+          uint8_t* dst = smem + st * kRStageBytes + part * kRHalf + box * p.box_rows * 128;
+          tma_load_4d(dst, part < 2 ? &tmK : &tmV, &full[st], (part & 1) * 64, key0 & bs_mask, at.h, c3);
+        }
+      }
+      left -= n;
+      if (left > 0 && !kv_next_unit<kRKT>(p, at)) break;
+    }
+    // Every copy has landed before the CTA may end (a consumer that gave up waits for none).
+    for (int k = max(0, it - kRStages); k < it; ++k)
+      if (!kv_wait(&full[k % kRStages], (k / kRStages) & 1, p.err)) break;
+    return;
+  }
+
+  // Consumers.
+  const uint32_t sbase = smem_u32(smem), jbase = smem_u32(join);
+  const int g = lane >> 2, cq = (lane & 3) * 2;  // accumulator row within 8, first of two columns
+  int it = 0;
+  bool ok = true;
+  while (left > 0) {
+    const int n = static_cast<int>(min(left, static_cast<int64_t>(at.n_tiles - at.tile)));
+    const int first = at.tile;
+    const int t0 = at.s.q0 + at.u * p.unit_tokens;
+    const int n_tok = min(p.unit_tokens, at.s.q_len - at.u * p.unit_tokens);
+    const int rows = n_tok * p.group;
+
+    // Q rows into shared memory (two halves of R rows x 128 bytes, 128-byte swizzle).
+    named_sync(1, 128);
+    for (int i = tid; i < R * 16; i += 128) {
+      const int r = i >> 4, ch = i & 15;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (r < rows) {
+        const int tok = r / p.group, hh = r - tok * p.group;
+        v = *reinterpret_cast<const uint4*>(p.q + static_cast<int64_t>(t0 + tok) * p.ld_q +
+                                            (static_cast<int64_t>(at.h) * p.group + hh) * 128 + ch * 8);
+      }
+      *reinterpret_cast<uint4*>(join + (ch >> 3) * (R * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = v;
+    }
+    named_sync(1, 128);
+    // A fragment (rows mt * 16.., channels ks * 16..).
+    auto load_q = [&](int mt, int ks, uint32_t (&a)[4]) {
+      const int r = mt * 16 + (lane & 15), ch = (ks & 3) * 2 + (lane >> 4);
+      ldsm4(jbase + (ks >> 2) * (R * 128) + r * 128 + ((ch ^ (r & 7)) << 4), a);
+    };
+    uint32_t qf[MT == 1 ? 8 : 1][4];
+    if constexpr (MT == 1) {
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) load_q(0, ks, qf[ks]);
+    }
+    // Keys each accumulator row attends to: [0, limit).
+    int limit[MT][2];
+    int min_limit = at.s.kv;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = mt * 16 + g + e * 8;
+        int lim = at.s.kv;
+        if (p.causal) lim = min(lim, at.s.off + at.u * p.unit_tokens + r / p.group + 1);
+        limit[mt][e] = lim;
+      }
+    if (p.causal) min_limit = min(min_limit, at.s.off + at.u * p.unit_tokens + 1);
+
+    float o[MT][16][4];
+    float m[MT][2], l[MT][2];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+      for (int d = 0; d < 16; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[mt][d][e] = 0.f;
+      m[mt][0] = m[mt][1] = -INFINITY;
+      l[mt][0] = l[mt][1] = 0.f;
+    }
+    for (int j = first; j < first + n; ++j, ++it) {
+      const int st = it % kRStages;
+      if (ok) ok = __all_sync(0xffffffffu, kv_wait(&full[st], (it / kRStages) & 1, p.err));
+      if (!ok) continue;  // a wait ran out: no more work, but every barrier below is still met
+      const int key0 = j * kRKT + warp * 16;
+      if (key0 < at.s.kv) {
+        const uint32_t kb = sbase + st * kRStageBytes, vb = kb + 2 * kRHalf;
+        const int krow = warp * 16 + ((lane >> 4) << 3) + (lane & 7);  // ldmatrix row of K
+        float s[MT][2][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[mt][nb][e] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) {
+          uint32_t b[4];
+          const int ch = (ks & 3) * 2 + ((lane >> 3) & 1);
+          ldsm4(kb + (ks >> 2) * kRHalf + krow * 128 + ((ch ^ (krow & 7)) << 4), b);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            if constexpr (MT == 1) {
+              mma16816<F16>(s[0][0], qf[ks], b[0], b[1]);
+              mma16816<F16>(s[0][1], qf[ks], b[2], b[3]);
+            } else {
+              uint32_t a[4];
+              load_q(mt, ks, a);
+              mma16816<F16>(s[mt][0], a, b[0], b[1]);
+              mma16816<F16>(s[mt][1], a, b[2], b[3]);
+            }
+          }
+        }
+        if (key0 + 16 > min_limit) {
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (key0 + nb * 8 + cq + (e & 1) >= limit[mt][e >> 1]) s[mt][nb][e] = -INFINITY;
+        }
+        uint32_t pf[MT][4];
+        bool grew = false;
+        float alpha[MT][2];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float mx = fmaxf(fmaxf(s[mt][0][2 * e], s[mt][0][2 * e + 1]), fmaxf(s[mt][1][2 * e], s[mt][1][2 * e + 1]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            mx *= p.scale_log2;
+            const float m_new = fmaxf(m[mt][e], mx);
+            const float ref = m_new == -INFINITY ? 0.f : m_new;  // no key so far: every numerator 0
+            grew |= m_new != m[mt][e];
+            alpha[mt][e] = kv_ex2(m[mt][e] - ref);
+            float sum = 0.f;
+#pragma unroll
+            for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+                float& x = s[mt][nb][2 * e + q];
+                x = kv_ex2(fmaf(x, p.scale_log2, -ref));
+                sum += x;
+              }
+            l[mt][e] = l[mt][e] * alpha[mt][e] + sum;
+            m[mt][e] = m_new;
+          }
+          pf[mt][0] = kv_pack2<F16>(s[mt][0][0], s[mt][0][1]);
+          pf[mt][1] = kv_pack2<F16>(s[mt][0][2], s[mt][0][3]);
+          pf[mt][2] = kv_pack2<F16>(s[mt][1][0], s[mt][1][1]);
+          pf[mt][3] = kv_pack2<F16>(s[mt][1][2], s[mt][1][3]);
+        }
+        if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int d = 0; d < 16; ++d)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[mt][d][e] *= alpha[mt][e >> 1];
+        }
+        const int vrow = warp * 16 + (((lane >> 3) & 1) << 3) + (lane & 7);  // ldmatrix row of V
+        if (key0 + 16 > at.s.kv) {
+          // Behind the last key a block holds anything, and 0 x NaN is NaN: clear those rows.
+          for (int i = lane; i < 256; i += 32) {
+            const int r = i >> 4, ch = i & 15;
+            if (key0 + r >= at.s.kv)
+              *reinterpret_cast<uint4*>(smem + st * kRStageBytes + (2 + (ch >> 3)) * kRHalf + (warp * 16 + r) * 128 +
+                                        ((ch & 7) << 4)) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();  // before a later TMA write to the same bytes
+          __syncwarp();
+        }
+#pragma unroll
+        for (int np = 0; np < 8; ++np) {
+          uint32_t b[4];
+          const int ch = (np & 3) * 2 + (lane >> 4);
+          ldsm4t(vb + (np >> 2) * kRHalf + vrow * 128 + ((ch ^ (vrow & 7)) << 4), b);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            mma16816<F16>(o[mt][2 * np], pf[mt], b[0], b[1]);
+            mma16816<F16>(o[mt][2 * np + 1], pf[mt], b[2], b[3]);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
+    }
+
+    // Join the four warps: weights 2^(m_w - M), sums over w in order.
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float x = l[mt][e];
+        x += __shfl_xor_sync(0xffffffffu, x, 1);
+        x += __shfl_xor_sync(0xffffffffu, x, 2);
+        if ((lane & 3) == 0) s_ml[warp][mt * 16 + g + e * 8] = make_float2(m[mt][e], x);
+      }
+    named_sync(1, 128);  // also: all Q fragments have been read
+    float w[MT][2];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = mt * 16 + g + e * 8;
+        const float M = fmaxf(fmaxf(s_ml[0][r].x, s_ml[1][r].x), fmaxf(s_ml[2][r].x, s_ml[3][r].x));
+        w[mt][e] = M == -INFINITY ? 0.f : kv_ex2(m[mt][e] - M);
+      }
+    const bool whole = first == 0 && n == at.n_tiles;
+    const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (first == 0 ? 1 : 0);
+    constexpr int DC = 32 / MT;               // output columns of a round
+    float* jf = reinterpret_cast<float*>(join);  // [warp][R][DC]
+#pragma unroll
+    for (int rd = 0; rd < 128 / DC; ++rd) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int d = 0; d < DC / 8; ++d)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float2 v = make_float2(o[mt][rd * (DC / 8) + d][2 * e] * w[mt][e],
+                                   o[mt][rd * (DC / 8) + d][2 * e + 1] * w[mt][e]);
+            *reinterpret_cast<float2*>(jf + (warp * R + mt * 16 + g + e * 8) * DC + d * 8 + cq) = v;
+          }
+      named_sync(1, 128);
+      const int r = tid / (DC / 4), c4 = (tid % (DC / 4)) * 4;
+      if (r < rows) {
+        float4 a = *reinterpret_cast<const float4*>(jf + r * DC + c4);
+#pragma unroll
+        for (int k = 1; k < 4; ++k) {
+          const float4 b = *reinterpret_cast<const float4*>(jf + (k * R + r) * DC + c4);
+          a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+        }
+        const float M = fmaxf(fmaxf(s_ml[0][r].x, s_ml[1][r].x), fmaxf(s_ml[2][r].x, s_ml[3][r].x));
+        float L = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) L += M == -INFINITY ? 0.f : s_ml[k][r].y * kv_ex2(s_ml[k][r].x - M);
+        if (whole) {
+          const float inv = L > 0.f ? 1.0f / L : 0.f;
+          const int tok = r / p.group, hh = r - tok * p.group;
+          uint16_t* dst = p.out + static_cast<int64_t>(t0 + tok) * p.ld_out +
+                          (static_cast<int64_t>(at.h) * p.group + hh) * 128 + rd * DC + c4;
+          *reinterpret_cast<uint2*>(dst) =
+              make_uint2(kv_pack2<F16>(a.x * inv, a.y * inv), kv_pack2<F16>(a.z * inv, a.w * inv));
+        } else {
+          *reinterpret_cast<float4*>(p.part_o + (slot * R + r) * 128 + rd * DC + c4) = a;
+          if (rd == 0 && c4 == 0) p.part_ml[slot * R + r] = make_float2(M, L);
+        }
+      }
+      named_sync(1, 128);
+    }
+    left -= n;
+    if (left > 0 && !kv_next_unit<kRKT>(p, at)) break;
+  }
+}
+
+// ------------------------------------------------------------ joining parts
+// Block c looks at the cut between parts c and c + 1.  If it goes through a unit
+// and is the first cut to do so, the block joins that unit's parts, in the order
+// of the parts: the result does not depend on which CTA finished first.
+constexpr int kJThreads = 256;
+
+template <int KT, int MIN_TILES, bool F16>
+__global__ void __launch_bounds__(kJThreads) kv_join_kernel(const __grid_constant__ KvAttnArgs p, int R) {
+  __shared__ KvSchedSmem<kJThreads> sched;
+  KvRange range;
+  KvPos at;
+  const int c = blockIdx.x + 1;
+  const bool have = kv_locate<KT, kJThreads, MIN_TILES>(p, sched, range, at, [&](const KvRange& r) {
+    return c < r.parts ? kv_cut(r, c) : static_cast<int64_t>(-1);
+  });
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!have || at.tile == 0) return;
+  const int64_t start = kv_cut(range, c) - at.tile;
+  if (kv_cut(range, c - 1) > start) return;  // an earlier cut went through this unit
+  const int64_t end = start + at.n_tiles;
+  int last = c;
+  while (last + 1 < range.parts && kv_cut(range, last + 1) < end) ++last;
+  const int t0 = at.s.q0 + at.u * p.unit_tokens;
+  const int rows = min(p.unit_tokens, at.s.q_len - at.u * p.unit_tokens) * p.group;
+  const int64_t first_slot = 2 * static_cast<int64_t>(c - 1) + 1;
+  for (int r = threadIdx.x >> 5; r < rows; r += kJThreads / 32) {
+    const int c4 = (threadIdx.x & 31) * 4;
+    float M = p.part_ml[first_slot * R + r].x;
+    for (int k = c; k <= last; ++k) M = fmaxf(M, p.part_ml[2 * static_cast<int64_t>(k) * R + r].x);
+    float L = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (M != -INFINITY) {
+      for (int k = c - 1; k <= last; ++k) {
+        const int64_t slot = k < c ? first_slot : 2 * static_cast<int64_t>(k);
+        const float2 ml = p.part_ml[slot * R + r];
+        const float4 b = *reinterpret_cast<const float4*>(p.part_o + (slot * R + r) * 128 + c4);
+        const float w = kv_ex2(ml.x - M);
+        L += w * ml.y;
+        a.x += w * b.x; a.y += w * b.y; a.z += w * b.z; a.w += w * b.w;
+      }
+    }
+    const float inv = L > 0.f ? 1.0f / L : 0.f;
+    const int tok = r / p.group, hh = r - tok * p.group;
+    uint16_t* dst = p.out + static_cast<int64_t>(t0 + tok) * p.ld_out +
+                    (static_cast<int64_t>(at.h) * p.group + hh) * 128 + c4;
+    *reinterpret_cast<uint2*>(dst) =
+        make_uint2(kv_pack2<F16>(a.x * inv, a.y * inv), kv_pack2<F16>(a.z * inv, a.w * inv));
+  }
+}
+
+// ------------------------------------------------------------------ host
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = [] {
+    void* q = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &q, cudaEnableDefault, &r) != cudaSuccess ||
+        r != cudaDriverEntryPointSuccess)
+      q = nullptr;
+    return reinterpret_cast<EncodeTiledFn>(q);
+  }();
+  return fn;
+}
+
+// One cache plane: {channel, token of the block, head, block}, boxes of 64 channels x box_rows tokens.
+cudaError_t cache_map(CUtensorMap* m, const KvCacheView& c, const void* base, int box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return cudaErrorNotSupported;
+  const cuuint64_t bs = static_cast<cuuint64_t>(c.block_size);
+  cuuint64_t dims[4] = {128, bs, static_cast<cuuint64_t>(c.heads_kv), static_cast<cuuint64_t>(c.n_blocks)};
+  cuuint64_t strides[3] = {256, bs * 256, static_cast<cuuint64_t>(c.block_stride) * 2};
+  cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows), 1, 1};
+  cuuint32_t es[4] = {1, 1, 1, 1};
+  const CUresult r =
+      fn(m, c.f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims,
+         strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+// Dynamic shared memory limit of a kernel, set once per device.
+template <class K>
+cudaError_t allow_smem(K* kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = uint64_t(1) << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
+
+template <int MT, bool F16>
+cudaError_t launch_rows(const KvCacheView& c, KvAttnArgs a, int grid, cudaStream_t s) {
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = allow_smem(kv_rows_kernel<MT, F16>, kRSmem, done);
+  if (e != cudaSuccess) return e;
+  a.box_rows = std::min(c.block_size, kRKT);
+  CUtensorMap mk, mv;
+  e = cache_map(&mk, c, c.k, a.box_rows);
+  if (e == cudaSuccess) e = cache_map(&mv, c, c.v, a.box_rows);
+  if (e != cudaSuccess) return e;
+  kv_rows_kernel<MT, F16><<<grid, kRThreads, kRSmem, s>>>(mk, mv, a);
+  return cudaGetLastError();
+}
+
+template <int KT, int MIN_TILES, bool F16>
+cudaError_t launch_join(const KvAttnArgs& a, int rows, cudaStream_t s) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(a.grid - 1);
+  cfg.blockDim = dim3(kJThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  // May start while the main kernel runs; waits for its end before it reads the parts.
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kv_join_kernel<KT, MIN_TILES, F16>, a, rows);
+}
+
+}  // namespace
+
+KvAttnPlan kv_attention_plan(int heads, int heads_kv, int64_t max_new, int num_sms) {
+  const int group = heads / heads_kv;
+  KvAttnPlan pl{};
+  pl.unit_rows = max_new * group <= 16 ? 16 : 32;
+  pl.unit_tokens = pl.unit_rows / group;
+  pl.grid = 2 * num_sms;
+  const size_t rows = 2 * static_cast<size_t>(pl.grid) * pl.unit_rows;
+  pl.ml_bytes = rows * sizeof(float2);  // a multiple of 16
+  pl.bytes = pl.ml_bytes + rows * 128 * sizeof(float);
+  return pl;
+}
+
+cudaError_t launch_kv_attention(const KvCacheView& c, KvAttnArgs a, const KvAttnPlan& plan, void* workspace,
+                                cudaStream_t s) {
+  a.unit_tokens = plan.unit_tokens;
+  a.grid = plan.grid;
+  a.part_ml = static_cast<float2*>(workspace);
+  a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan.ml_bytes);
+  cudaError_t e;
+  if (plan.unit_rows == 16)
+    e = c.f16 ? launch_rows<1, true>(c, a, plan.grid, s) : launch_rows<1, false>(c, a, plan.grid, s);
+  else
+    e = c.f16 ? launch_rows<2, true>(c, a, plan.grid, s) : launch_rows<2, false>(c, a, plan.grid, s);
+  if (e != cudaSuccess) return e;
+  return c.f16 ? launch_join<kRKT, kRMinTiles, true>(a, plan.unit_rows, s)
+               : launch_join<kRKT, kRMinTiles, false>(a, plan.unit_rows, s);
+}
+
+}  // namespace dcpp

@@ -1,0 +1,203 @@
+// How the paged attention kernels share out their work.
+//
+// A sequence's query rows are cut into units of `unit_tokens` tokens; a unit of
+// one key / value head has n(u) key tiles of KT keys (causal: up to its last
+// token's position).  All (sequence, head, unit, tile) quadruples in this order
+// form one line of `total` tiles, cut into equal runs, one for each CTA, so that
+// any mix of lengths fills the GPU evenly.  A unit that a cut goes through is
+// computed in parts by neighbouring CTAs and joined afterwards.  Lengths live on
+// the device: every CTA sums them for itself (no plan launch, nothing to keep
+// between calls), and every quantity here is a function of them alone.
+#pragma once
+
+#include "common.cuh"
+#include "kv_cache.cuh"
+
+namespace dcpp {
+
+// sum_{i < n} floor((a i + b) / m): the Euclid-like floor-sum recurrence (as in
+// the AtCoder Library's floor_sum).  All values below 2^31.
+__device__ __forceinline__ int64_t kv_floor_sum(int64_t n, uint32_t m, uint32_t a, uint32_t b) {
+  int64_t ans = 0;
+  uint32_t nn = static_cast<uint32_t>(n);
+  while (nn > 0) {
+    if (a >= m) {
+      ans += static_cast<int64_t>(nn) * (nn - 1) / 2 * (a / m);
+      a %= m;
+    }
+    if (b >= m) {
+      ans += static_cast<int64_t>(nn) * (b / m);
+      b %= m;
+    }
+    const uint64_t top = static_cast<uint64_t>(a) * nn + b;
+    if (top < m) break;
+    nn = static_cast<uint32_t>(top / m);
+    b = static_cast<uint32_t>(top % m);
+    const uint32_t t = m;
+    m = a;
+    a = t;
+  }
+  return ans;
+}
+
+// One sequence's share of the work.
+struct KvSeq {
+  int32_t q0, q_len;  // its rows in q
+  int32_t kv;         // cached keys
+  int32_t off;        // position of its first new token: kv - q_len (negative: no key for it)
+  int32_t units;
+};
+
+// Lengths out of range record an error and leave the sequence out.
+__device__ __forceinline__ KvSeq kv_seq(const KvAttnArgs& p, int b) {
+  KvSeq s;
+  const int32_t c0 = p.cu_new[b], c1 = p.cu_new[b + 1];
+  s.kv = p.seq_lens[b];
+  s.q0 = c0;
+  s.q_len = c1 - c0;
+  if (c0 < 0 || c1 < c0 || c1 > p.tokens || s.q_len > p.max_new || s.kv < 0 || s.kv > p.max_kv) {
+    record_error(p.err, kDevBadCache);
+    s.q0 = s.q_len = s.kv = 0;
+  }
+  s.off = s.kv - s.q_len;
+  s.units = (s.q_len + p.unit_tokens - 1) / p.unit_tokens;
+  return s;
+}
+
+// Key tiles of unit u: at least one, so that a unit without keys still writes its zeros.
+template <int KT>
+__device__ __forceinline__ int kv_unit_tiles(const KvAttnArgs& p, const KvSeq& s, int u) {
+  int keys = s.kv;
+  if (p.causal) keys = min(keys, s.off + (u + 1) * p.unit_tokens);
+  return max(1, (keys + KT - 1) / KT);
+}
+
+// sum_{v < u} n(v).
+template <int KT>
+__device__ __forceinline__ int64_t kv_units_before(const KvAttnArgs& p, const KvSeq& s, int u) {
+  if (u <= 0) return 0;
+  const int full = max(1, (s.kv + KT - 1) / KT);
+  if (!p.causal) return static_cast<int64_t>(u) * full;
+  int64_t sum = 0;
+  int n = u;
+  if (u == s.units) {  // the last unit may end before unit_tokens tokens
+    sum = full;
+    --n;
+  }
+  // Units whose last key lies in the first tile (or before it) count 1.
+  const int U = p.unit_tokens;
+  const int ones = s.off + U > KT ? 0 : min(n, (KT - s.off) / U);
+  sum += ones;
+  if (n > ones)
+    sum += kv_floor_sum(n - ones, KT, static_cast<uint32_t>(U),
+                        static_cast<uint32_t>(s.off + (ones + 1) * U + KT - 1));
+  return sum;
+}
+
+struct KvPos {
+  KvSeq s;
+  int32_t b, h, u;
+  int32_t tile, n_tiles;  // current tile of the unit, tiles of the unit
+};
+
+struct KvRange {
+  int64_t total;  // tiles in all
+  int32_t parts;  // CTAs that have work
+};
+
+// Shared memory of the schedule: per-thread tile sums and the position found.
+template <int NT>
+struct KvSchedSmem {
+  int64_t warp[NT / 32];
+  int64_t base;
+  int32_t b;
+};
+
+// First tile of part i of r.parts.
+__device__ __forceinline__ int64_t kv_cut(const KvRange& r, int i) { return r.total * i / r.parts; }
+
+// All NT threads of the block: the total, and the position of the tile at
+// pos_of(range) on the line (pos_of may return a value outside [0, total): no
+// position, false).  MIN_TILES: fewest tiles of a part.
+template <int KT, int NT, int MIN_TILES, class PosOf>
+__device__ __forceinline__ bool kv_locate(const KvAttnArgs& p, KvSchedSmem<NT>& sm, KvRange& r, KvPos& at, PosOf pos_of) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int seg = (p.batch + NT - 1) / NT;
+  const int b0 = min(tid * seg, p.batch), b1 = min(b0 + seg, p.batch);
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b) {
+    const KvSeq s = kv_seq(p, b);
+    mine += kv_units_before<KT>(p, s, s.units) * p.heads_kv;
+  }
+  int64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t u = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += u;
+  }
+  if (lane == 31) sm.warp[warp] = incl;
+  __syncthreads();
+  int64_t before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < NT / 32; ++w) {
+    if (w < warp) before += sm.warp[w];
+    total += sm.warp[w];
+  }
+  r.total = total;
+  r.parts = static_cast<int>(max(static_cast<int64_t>(1), min(static_cast<int64_t>(p.grid), total / MIN_TILES)));
+  const int64_t pos = pos_of(r);
+  if (pos < 0 || pos >= total) return false;
+  int64_t base = before + incl - mine;
+  if (pos >= base && pos < base + mine) {
+    for (int b = b0; b < b1; ++b) {
+      const KvSeq s = kv_seq(p, b);
+      const int64_t n = kv_units_before<KT>(p, s, s.units) * p.heads_kv;
+      if (pos < base + n) {
+        sm.b = b;
+        sm.base = base;
+        break;
+      }
+      base += n;
+    }
+  }
+  __syncthreads();
+  at.b = sm.b;
+  at.s = kv_seq(p, at.b);
+  const int64_t per_head = kv_units_before<KT>(p, at.s, at.s.units);
+  int64_t rem = pos - sm.base;
+  at.h = static_cast<int>(rem / per_head);
+  rem -= at.h * per_head;
+  int lo = 0, hi = at.s.units;  // units_before(lo) <= rem < units_before(hi)
+  while (hi - lo > 1) {
+    const int step = (hi - lo + NT - 1) / NT;
+    const int64_t cand = static_cast<int64_t>(lo) + static_cast<int64_t>(tid) * step;
+    const bool in = cand < hi && kv_units_before<KT>(p, at.s, static_cast<int>(min(cand, static_cast<int64_t>(hi)))) <= rem;
+    const int k = __syncthreads_count(in);  // thread 0 always counts
+    lo += (k - 1) * step;
+    hi = min(hi, lo + step);
+  }
+  at.u = lo;
+  at.tile = static_cast<int>(rem - kv_units_before<KT>(p, at.s, lo));
+  at.n_tiles = kv_unit_tiles<KT>(p, at.s, lo);
+  return true;
+}
+
+// The next unit on the line (false: there is none).
+template <int KT>
+__device__ __forceinline__ bool kv_next_unit(const KvAttnArgs& p, KvPos& at) {
+  at.tile = 0;
+  if (++at.u >= at.s.units) {
+    at.u = 0;
+    if (++at.h >= p.heads_kv) {
+      at.h = 0;
+      do {
+        if (++at.b >= p.batch) return false;
+        at.s = kv_seq(p, at.b);
+      } while (at.s.units == 0);
+    }
+  }
+  at.n_tiles = kv_unit_tiles<KT>(p, at.s, at.u);
+  return true;
+}
+
+}  // namespace dcpp

@@ -145,6 +145,9 @@ const char* device_error_name(int code) {
     case kDevTimeoutAttn: return "attention pipeline wait timed out";
     case kDevTimeoutPeer: return "tensor-parallel barrier timed out waiting for a peer GPU";
     case kDevBadIndex: return "token id outside the embedding table";
+    case kDevBadCache: return "paged cache: a length, block id or slot is out of range";
+    case kDevNoBlocks: return "paged cache: the step needs more free blocks or token rows than there are";
+    case kDevTimeoutKv: return "paged attention pipeline wait timed out";
     default: return "unknown device error";
   }
 }
@@ -155,7 +158,11 @@ void Ctx::check_device_error() {
   cuda_check(cudaStreamSynchronize(stream), "cudaStreamSynchronize");
   if (h != 0) {
     cuda_check(cudaMemsetAsync(d_err, 0, sizeof(int), stream), "clear error word");
-    fail(h == kDevBadShape ? DCPP_ERR_UNSUPPORTED : (h == kDevBadIndex ? DCPP_ERR_INVALID_ARG : DCPP_ERR_TIMEOUT),
+    dcpp_status st = DCPP_ERR_TIMEOUT;
+    if (h == kDevBadShape) st = DCPP_ERR_UNSUPPORTED;
+    if (h == kDevBadIndex || h == kDevBadCache) st = DCPP_ERR_INVALID_ARG;
+    if (h == kDevNoBlocks) st = DCPP_ERR_OOM;
+    fail(st,
          std::string("device error ") + std::to_string(h) + ": " + device_error_name(h));
   }
 }

@@ -108,6 +108,20 @@ class VAEConfigC(ctypes.Structure):
     ]
 
 
+class KVCacheC(ctypes.Structure):
+    """dcpp_kv_cache."""
+    _fields_ = [
+        ("type", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+        ("n_blocks", ctypes.c_int64),
+        ("heads_kv", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64),
+        ("block_stride", ctypes.c_int64),
+        ("d_k", ctypes.c_void_p),
+        ("d_v", ctypes.c_void_p),
+    ]
+
+
 # name -> (restype, argtypes)
 _SIGNATURES = {
     "dcpp_version": (ctypes.c_char_p, []),
@@ -138,6 +152,15 @@ _SIGNATURES = {
     "dcpp_layernorm_mod": (ctypes.c_int, [_vp, _vp, ctypes.c_int64, ctypes.c_int64, _vp, _vp, ctypes.c_float, _vp]),
     "dcpp_attention": (ctypes.c_int, [_vp, _vp, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _vp, _vp,
                                       ctypes.c_float, _vp, ctypes.c_int, _c_i64p, ctypes.c_float, _vp]),
+    "dcpp_kv_plan": (ctypes.c_int, [_vp, _vp, ctypes.c_int64, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_int64, _vp, _vp,
+                                    ctypes.c_int64, _vp, _vp]),
+    "dcpp_kv_store": (ctypes.c_int, [_vp, _vp, ctypes.c_int64, ctypes.c_int64, _vp, ctypes.c_int64, _vp, _vp, ctypes.c_float,
+                                     ctypes.c_int, ctypes.c_float, _vp, _vp, _vp, ctypes.c_int64]),
+    "dcpp_kv_attention_workspace": (ctypes.c_int, [_vp, _vp, ctypes.c_int64, ctypes.c_int64,
+                                                   ctypes.POINTER(ctypes.c_size_t)]),
+    "dcpp_kv_attention": (ctypes.c_int, [_vp, _vp, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _vp, ctypes.c_int64, _vp,
+                                         _vp, _vp, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_float, _vp,
+                                         ctypes.c_size_t, _vp, ctypes.c_int64]),
     "dcpp_flux2_config_default": (None, [ctypes.POINTER(Flux2ConfigC)]),
     "dcpp_flux2_config_from_file": (ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(Flux2ConfigC)]),
     "dcpp_flux2_create": (ctypes.c_int, [_vp, ctypes.POINTER(Flux2ConfigC), ctypes.POINTER(_vp)]),
@@ -264,6 +287,61 @@ def _ptr(x) -> Optional[int]:
     raise TypeError(f"cannot take the address of {type(x)}")
 
 
+def _rows(x, device: int, type_: int, cols: int, what: str):
+    """(address, rows, row stride) of a 2-D or 3-D torch tensor of 16-bit rows on
+    `device` whose trailing dimensions are packed and hold `cols` values."""
+    if x.get_device() != device or x.dtype != _torch_dtype(type_):
+        raise DcppError(DCPP_ERR_INVALID_ARG, f"{what}: must be a {_torch_dtype(type_)} tensor on cuda:{device}")
+    shape, stride = x.shape, x.stride()
+    packed = (len(shape) == 2 and stride[1] == 1 or
+              len(shape) == 3 and stride[2] == 1 and (stride[1] == shape[2] or shape[1] == 1))
+    if not packed or x.numel() != shape[0] * cols:
+        raise DcppError(DCPP_ERR_INVALID_ARG, f"{what}: must be rows of {cols} packed values")
+    return x.data_ptr(), shape[0], stride[0] if shape[0] > 1 else max(stride[0], cols)
+
+
+def _vec(x, device: int, dtype: str, n: Optional[int], what: str):
+    """Address of a packed torch tensor of `n` values (None: any number) on `device`."""
+    if x.get_device() != device or str(x.dtype) != dtype or not x.is_contiguous() or (n is not None and x.numel() != n):
+        raise DcppError(DCPP_ERR_INVALID_ARG, f"{what}: must be a packed {dtype} tensor on cuda:{device}"
+                        + ("" if n is None else f" of {n} values"))
+    return x.data_ptr()
+
+
+def _torch_dtype(type_: int):
+    import torch
+    return torch.float16 if type_ == TYPE_F16 else torch.bfloat16
+
+
+class KVCache:
+    """dcpp_kv_cache: one layer's paged key / value cache over torch tensors k, v
+    [n_blocks, heads_kv, block_size, 128] (bf16 or f16; each block packed, any block
+    stride, the same for both).  Without tensors, only the geometry that kv_plan
+    needs: KVCache(n_blocks=..., block_size=...)."""
+
+    def __init__(self, k=None, v=None, n_blocks: int = 0, block_size: int = 0):
+        c = KVCacheC()
+        if k is not None:
+            import torch
+            if v is None or k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride() or \
+                    not k.is_cuda or k.device != v.device or k.dtype not in (torch.bfloat16, torch.float16):
+                raise DcppError(DCPP_ERR_INVALID_ARG, "KVCache: k and v must be bf16 or f16 CUDA tensors [n_blocks, "
+                                "heads_kv, block_size, 128] of one layout")
+            nb, h, bs, d = k.shape
+            if k.stride()[1:] != (bs * d, d, 1):
+                raise DcppError(DCPP_ERR_INVALID_ARG, "KVCache: the heads, tokens and channels of a block must be packed")
+            c.type = TYPE_F16 if k.dtype == torch.float16 else TYPE_BF16
+            c.block_size, c.n_blocks, c.heads_kv, c.head_dim, c.block_stride = bs, nb, h, d, max(k.stride(0), h * bs * d)
+            c.d_k, c.d_v = k.data_ptr(), v.data_ptr()
+            self.device = k.get_device()
+        else:
+            c.block_size, c.n_blocks = block_size, n_blocks
+            self.device = None
+        self.k, self.v = k, v  # keeps the storage alive
+        self.c = c
+        self.ref = ctypes.addressof(c)
+
+
 class Context:
     """dcpp_ctx: one GPU, one stream."""
 
@@ -322,6 +400,15 @@ class Context:
             own = self._own_stream.cuda_stream if self._own_stream is not None else None
             self.check(lib().dcpp_set_stream(self.h, own), "set_stream")
             self._stream = self._own_stream
+
+    def use_current_stream(self):
+        """Run on torch's current stream, the default stream included: calls made
+        while it stays current need no ordering events."""
+        import torch
+        s = torch.cuda.current_stream(self.device)
+        # The default stream's handle is 0, which the library reads as "its own": name it cudaStreamLegacy.
+        self.check(lib().dcpp_set_stream(self.h, s.cuda_stream or 1), "set_stream")
+        self._stream = s
 
     def _call(self, fn, *args):
         """fn(*args) (a C entry point that reads or writes device memory),
@@ -396,6 +483,76 @@ class Context:
         arr = (ctypes.c_int64 * len(axes_dims))(*axes_dims)
         self.check(self._call(lib().dcpp_attention, self.h, _ptr(qkv), B, S, H, 128, _ptr(norm_q), _ptr(norm_k), eps, _ptr(ids),
                                         len(axes_dims), arr, theta, _ptr(out)), "attention")
+
+    # paged key / value cache (torch tensors on the context's GPU)
+    ROPE = {"none": 0, "normal": 1, "neox": 2}
+
+    def _on_device(self, cache: "KVCache", what: str):
+        if cache.device != self.device:
+            raise DcppError(DCPP_ERR_INVALID_ARG, f"{what}: the cache is not on cuda:{self.device}")
+
+    def kv_plan(self, cache: "KVCache", cached, new, free_blocks, free_in, free_out, block_table, seq_lens, cu_new, slots,
+                positions):
+        """Plan one step of cached.numel() requests (dcpp_kv_plan): block_table
+        [batch, max_blocks], slots / positions [max_tokens]."""
+        d, batch, rows = self.device, cached.numel(), slots.numel()
+        i32, i64 = "torch.int32", "torch.int64"
+        if block_table.dim() != 2 or block_table.shape[0] != batch:
+            raise DcppError(DCPP_ERR_INVALID_ARG, "kv_plan: block_table must be [batch, max_blocks]")
+        self.check(self._call(
+            lib().dcpp_kv_plan, self.h, cache.ref, batch, _vec(cached, d, i32, batch, "cached"),
+            _vec(new, d, i32, batch, "new"), _vec(free_blocks, d, i32, cache.c.n_blocks, "free_blocks"),
+            _vec(free_in, d, i64, 2, "free_in"), _vec(free_out, d, i64, 2, "free_out"),
+            _vec(block_table, d, i32, None, "block_table"), block_table.shape[1], _vec(seq_lens, d, i32, batch, "seq_lens"),
+            _vec(cu_new, d, i32, batch + 1, "cu_new"), rows, _vec(slots, d, i32, rows, "slots"),
+            _vec(positions, d, i32, rows, "positions")), "kv_plan")
+
+    def kv_store(self, cache: "KVCache", qkv, heads: int, positions, slots, q, norm_q=None, norm_k=None, eps: float = 1e-6,
+                 rope: str = "neox", theta: float = 1e6):
+        """RMSNorm + rotary embedding of q and k, k and v into the cache (dcpp_kv_store).
+        qkv [tokens, (heads + 2 heads_kv) * 128] and q [tokens, heads(, )* 128] may be row-strided."""
+        d, c = self.device, cache.c
+        self._on_device(cache, "kv_store")
+        src, rows, ld = _rows(qkv, d, c.type, (heads + 2 * c.heads_kv) * 128, "qkv")
+        dst, rows_q, ld_q = _rows(q, d, c.type, heads * 128, "q")
+        if rows_q != rows or rope not in self.ROPE:
+            raise DcppError(DCPP_ERR_INVALID_ARG, "kv_store: q must have qkv's rows; rope is 'none', 'normal' or 'neox'")
+        f32, i32 = "torch.float32", "torch.int32"
+        self.check(self._call(
+            lib().dcpp_kv_store, self.h, cache.ref, rows, heads, src, ld,
+            None if norm_q is None else _vec(norm_q, d, f32, 128, "norm_q"),
+            None if norm_k is None else _vec(norm_k, d, f32, 128, "norm_k"), eps, self.ROPE[rope], theta,
+            None if positions is None else _vec(positions, d, i32, rows, "positions"), _vec(slots, d, i32, rows, "slots"),
+            dst, ld_q), "kv_store")
+
+    def kv_attention_workspace(self, cache: "KVCache", heads: int, max_new: int) -> int:
+        """Bytes of the workspace kv_attention needs (dcpp_kv_attention_workspace)."""
+        out = ctypes.c_size_t()
+        self.check(lib().dcpp_kv_attention_workspace(self.h, cache.ref, heads, max_new, ctypes.byref(out)),
+                   "kv_attention_workspace")
+        return out.value
+
+    def kv_attention(self, cache: "KVCache", q, cu_new, seq_lens, block_table, max_new: int, workspace, out,
+                     causal: bool = True, scale: Optional[float] = None):
+        """Attention of the new tokens over the cache (dcpp_kv_attention): q, out
+        [tokens, heads, 128], rows may be strided; scale None: 1 / sqrt(128)."""
+        d, c = self.device, cache.c
+        self._on_device(cache, "kv_attention")
+        if q.dim() != 3 or q.shape != out.shape:
+            raise DcppError(DCPP_ERR_INVALID_ARG, "kv_attention: q and out must be [tokens, heads, 128]")
+        heads, batch = q.shape[1], seq_lens.numel()
+        src, rows, ld = _rows(q, d, c.type, heads * 128, "q")
+        dst, _, ld_out = _rows(out, d, c.type, heads * 128, "out")
+        if block_table.dim() != 2 or block_table.shape[0] != batch:
+            raise DcppError(DCPP_ERR_INVALID_ARG, "kv_attention: block_table must be [batch, max_blocks]")
+        if workspace.get_device() != d or not workspace.is_contiguous():
+            raise DcppError(DCPP_ERR_INVALID_ARG, f"kv_attention: the workspace must be packed, on cuda:{d}")
+        i32 = "torch.int32"
+        self.check(self._call(
+            lib().dcpp_kv_attention, self.h, cache.ref, batch, rows, heads, src, ld, _vec(cu_new, d, i32, batch + 1, "cu_new"),
+            _vec(seq_lens, d, i32, batch, "seq_lens"), _vec(block_table, d, i32, None, "block_table"), block_table.shape[1],
+            max_new, 1 if causal else 0, 128.0 ** -0.5 if scale is None else scale, workspace.data_ptr(), workspace.nbytes,
+            dst, ld_out), "kv_attention")
 
     # tensor parallelism
     @staticmethod

@@ -211,6 +211,104 @@ dcpp_status dcpp_attention(dcpp_ctx* ctx, const uint16_t* d_qkv, int64_t B, int6
                            uint16_t* d_out);
 
 /* ---------------------------------------------------------------------- */
+/* Paged key / value cache: requests that grow token by token              */
+/* ---------------------------------------------------------------------- */
+
+/* The reference keeps no cache: its Qwen3 forward (Qwen3Model.cpp:99-208) is
+ * a prefill over whole prompts.  These entry points let prompts of different
+ * lengths share one cache, grow by chunks or single tokens, and attend to what
+ * is cached.  A step is plan -> (projection) -> store -> attention; lengths,
+ * block ids and maps stay on the device, so a step can be captured in a graph
+ * and replayed with other lengths.
+ *
+ * The cache holds n_blocks blocks of block_size tokens of every key / value
+ * head; request b's token p is token p % block_size of block
+ * block_table[b][p / block_size].  One descriptor serves one layer. */
+typedef struct dcpp_kv_cache {
+    int32_t type;          /* DCPP_TYPE_BF16 or DCPP_TYPE_F16 */
+    int32_t block_size;    /* tokens per block: 16, 32, 64, 128 or 256 */
+    int64_t n_blocks;      /* n_blocks * block_size < 2^31 */
+    int64_t heads_kv;
+    int64_t head_dim;      /* 128 */
+    int64_t block_stride;  /* elements between blocks of d_k (and of d_v), a multiple of 8; 0: packed */
+    void* d_k;             /* [n_blocks][heads_kv, block_size, head_dim], 16-byte aligned */
+    void* d_v;             /* the same */
+} dcpp_kv_cache;
+
+/* Plan one step of `batch` requests (at most 8192), on the GPU, from their
+ * lengths: d_cached[b] tokens are in the cache, d_new[b] are added; d_new[b] < 0
+ * marks a finished request, whose blocks are given back.
+ *   d_free_blocks  [n_blocks] ring of free block ids; d_free_in = {head, tail}
+ *                  counters: ring entries head .. tail - 1 (mod n_blocks) are
+ *                  free.  New blocks are taken from head in request order,
+ *                  returned ones go behind tail in request order (and are free
+ *                  from the next step on).  d_free_out gets the counters after
+ *                  the step and may be d_free_in.
+ *   d_block_table  [batch, max_blocks]: entries of new blocks are written,
+ *                  others left as they are.
+ *   d_seq_lens     [batch] tokens after the step (0: finished); may be d_cached.
+ *   d_cu_new       [batch + 1] row offsets of the requests' new tokens.
+ *   d_slots, d_positions  [max_tokens] cache slot (block * block_size + offset)
+ *                  and position of every new token; rows behind the last one get
+ *                  slot -1 and position 0.
+ * Of the cache only block_size and n_blocks are used.  A step that does not fit
+ * (free blocks, max_blocks, max_tokens) or whose lengths or counters make no
+ * sense is refused as a whole: cu_new 0, slots -1, seq_lens = cached, counters
+ * and table unchanged; dcpp_synchronize reports DCPP_ERR_OOM or
+ * DCPP_ERR_INVALID_ARG.  Outputs must not overlap the other arrays. */
+dcpp_status dcpp_kv_plan(dcpp_ctx* ctx, const dcpp_kv_cache* cache, int64_t batch, const int32_t* d_cached,
+                         const int32_t* d_new, int32_t* d_free_blocks, const int64_t* d_free_in, int64_t* d_free_out,
+                         int32_t* d_block_table, int64_t max_blocks, int32_t* d_seq_lens, int32_t* d_cu_new,
+                         int64_t max_tokens, int32_t* d_slots, int32_t* d_positions);
+
+/* Pairs that the rotary embedding turns. */
+#define DCPP_ROPE_NONE 0
+#define DCPP_ROPE_NORMAL 1 /* channels 2i, 2i + 1 */
+#define DCPP_ROPE_NEOX 2   /* channels i, i + 64 (Qwen3) */
+
+/* The attention prologue of a step's rows (RMSNorm.cpp:12-22, then rotary
+ * embedding by position), written where attention reads it:
+ *   qkv  [tokens, (heads + 2 heads_kv) * 128] projection rows q | k | v of the
+ *        cache's type, row stride ld_qkv elements
+ *   q    <- rope(RMSNorm(q) * norm_q), [tokens, heads * 128], row stride ld_q;
+ *        may be qkv's own q columns (d_q == d_qkv, ld_q == ld_qkv)
+ *   k    <- rope(RMSNorm(k) * norm_k) into the cache at d_slots, v as it is
+ * norm_q / norm_k [128] f32, NULL: no normalisation.  Pair i turns by position *
+ * theta^(-i / 64), the angle in 64 bits.  Rows with slot < 0 are skipped (q too);
+ * a slot outside the cache is skipped and reported by dcpp_synchronize
+ * (DCPP_ERR_INVALID_ARG).  Slots must be distinct.  Rows and planes: 16-byte
+ * aligned, strides multiples of 8. */
+dcpp_status dcpp_kv_store(dcpp_ctx* ctx, const dcpp_kv_cache* cache, int64_t tokens, int64_t heads,
+                          const uint16_t* d_qkv, int64_t ld_qkv, const float* d_norm_q, const float* d_norm_k,
+                          float eps, int rope, float theta, const int32_t* d_positions, const int32_t* d_slots,
+                          uint16_t* d_q, int64_t ld_q);
+
+/* Attention of the new tokens over the cache: row t of request b (rows
+ * cu_new[b] .. cu_new[b + 1] - 1) attends to the request's seq_lens[b] cached
+ * tokens, with `causal` only up to its own position
+ * (seq_lens[b] - its new tokens + t - cu_new[b]); out = softmax(scale q k^T) v,
+ * query head h reading key / value head h / (heads / heads_kv).  A row that
+ * attends to nothing is 0.  causal = 0 also serves as cross attention to states
+ * of another length.
+ *   q, out  [tokens, heads, 128] of the cache's type, row strides ld_q, ld_out;
+ *           rows of no request are left as they were
+ *   max_new at least every request's number of new tokens (picks the kernel)
+ *   workspace  dcpp_kv_attention_workspace bytes, 16-byte aligned; need not be
+ *           cleared, keeps nothing between calls; calls that may run at the same
+ *           time (other streams, graphs replayed side by side) need their own
+ * Block table entries beyond a request's tokens, and what its last block holds
+ * behind them, are never used.  Lengths or block ids out of range leave the
+ * request's rows undefined and are reported by dcpp_synchronize
+ * (DCPP_ERR_INVALID_ARG).  Up to 32 query heads per key / value head. */
+dcpp_status dcpp_kv_attention_workspace(dcpp_ctx* ctx, const dcpp_kv_cache* cache, int64_t heads, int64_t max_new,
+                                        size_t* out_bytes);
+dcpp_status dcpp_kv_attention(dcpp_ctx* ctx, const dcpp_kv_cache* cache, int64_t batch, int64_t tokens, int64_t heads,
+                              const uint16_t* d_q, int64_t ld_q, const int32_t* d_cu_new, const int32_t* d_seq_lens,
+                              const int32_t* d_block_table, int64_t max_blocks, int64_t max_new, int causal,
+                              float scale, void* d_workspace, size_t workspace_bytes, uint16_t* d_out,
+                              int64_t ld_out);
+
+/* ---------------------------------------------------------------------- */
 /* Model-level entry points: Flux2Transformer2DModel + Euler step          */
 /* ---------------------------------------------------------------------- */
 
