@@ -1,4 +1,5 @@
 // C ABI of the paged key / value cache: argument checks and launches.
+#include <algorithm>
 #include <cmath>
 
 #include "kv_cache.cuh"
@@ -190,7 +191,7 @@ dcpp_status dcpp_kv_attention_workspace(dcpp_ctx* ctx, const dcpp_kv_cache* cach
     if (!out_bytes) bad(kName, "null output");
     check_cache(cache, kName, true);
     check_attention_shape(*cache, heads, max_new, kName);
-    *out_bytes = dcpp::kv_attention_plan(static_cast<int>(heads), static_cast<int>(cache->heads_kv), max_new, ctx->num_sms).bytes;
+    *out_bytes = dcpp::kv_attention_plan(static_cast<int>(heads), static_cast<int>(cache->heads_kv), std::min<int64_t>(max_new, 1 << 24), ctx->num_sms).bytes;
   });
 }
 
@@ -216,7 +217,7 @@ dcpp_status dcpp_kv_attention(dcpp_ctx* ctx, const dcpp_kv_cache* cache, int64_t
     if (overlap(d_q, (tokens - 1) * ld_q + cols, d_out, (tokens - 1) * ld_out + cols)) bad(kName, "out must be apart from q");
     if (!d_cu_new || !d_seq_lens || !d_block_table) bad(kName, "null pointer");
     const dcpp::KvAttnPlan plan =
-        dcpp::kv_attention_plan(static_cast<int>(heads), static_cast<int>(cache->heads_kv), max_new, ctx->num_sms);
+        dcpp::kv_attention_plan(static_cast<int>(heads), static_cast<int>(cache->heads_kv), std::min<int64_t>(max_new, 1 << 24), ctx->num_sms);
     if (!d_workspace || !aligned(d_workspace, 16) || workspace_bytes < plan.bytes)
       bad(kName, ("needs a 16-byte aligned workspace of " + std::to_string(plan.bytes) + " bytes").c_str());
     a.q = d_q;

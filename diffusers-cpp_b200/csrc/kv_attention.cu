@@ -8,44 +8,14 @@
 //
 // Rows of one key / value head: the `group` query heads that share it times the
 // tokens of a unit, so that K and V are read once for all of them.
+#include "kv_device.cuh"
 #include "kv_sched.cuh"
 
 #include <algorithm>
-#include <atomic>
 
 namespace dcpp {
 
 namespace {
-
-__device__ __forceinline__ float kv_ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-template <bool F16>
-__device__ __forceinline__ uint32_t kv_pack2(float lo, float hi) {
-  if constexpr (F16) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  } else {
-    return pack_bf16x2(lo, hi);
-  }
-}
-
-// Bounded wait that looks at nothing but its barrier and the clock: another
-// kernel's recorded error does not end this one's work.
-__device__ __forceinline__ bool kv_wait(uint64_t* bar, uint32_t parity, int* err) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const unsigned long long t0 = globaltimer();
-  for (;;) {
-    if (mbar_try_wait_sleep(bar, parity, 20000u)) return true;
-    if (globaltimer() - t0 > kWaitTimeoutNs) {
-      record_error(err, kDevTimeoutKv);
-      return false;
-    }
-  }
-}
 
 __device__ __forceinline__ void named_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
@@ -292,14 +262,14 @@ __global__ void __launch_bounds__(kRThreads, 2)
             const float m_new = fmaxf(m[mt][e], mx);
             const float ref = m_new == -INFINITY ? 0.f : m_new;  // no key so far: every numerator 0
             grew |= m_new != m[mt][e];
-            alpha[mt][e] = kv_ex2(m[mt][e] - ref);
+            alpha[mt][e] = ex2(m[mt][e] - ref);
             float sum = 0.f;
 #pragma unroll
             for (int nb = 0; nb < 2; ++nb)
 #pragma unroll
               for (int q = 0; q < 2; ++q) {
                 float& x = s[mt][nb][2 * e + q];
-                x = kv_ex2(fmaf(x, p.scale_log2, -ref));
+                x = ex2(fmaf(x, p.scale_log2, -ref));
                 sum += x;
               }
             l[mt][e] = l[mt][e] * alpha[mt][e] + sum;
@@ -364,7 +334,7 @@ __global__ void __launch_bounds__(kRThreads, 2)
       for (int e = 0; e < 2; ++e) {
         const int r = mt * 16 + g + e * 8;
         const float M = fmaxf(fmaxf(s_ml[0][r].x, s_ml[1][r].x), fmaxf(s_ml[2][r].x, s_ml[3][r].x));
-        w[mt][e] = M == -INFINITY ? 0.f : kv_ex2(m[mt][e] - M);
+        w[mt][e] = M == -INFINITY ? 0.f : ex2(m[mt][e] - M);
       }
     const bool whole = first == 0 && n == at.n_tiles;
     const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (first == 0 ? 1 : 0);
@@ -394,7 +364,7 @@ __global__ void __launch_bounds__(kRThreads, 2)
         const float M = fmaxf(fmaxf(s_ml[0][r].x, s_ml[1][r].x), fmaxf(s_ml[2][r].x, s_ml[3][r].x));
         float L = 0.f;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) L += M == -INFINITY ? 0.f : s_ml[k][r].y * kv_ex2(s_ml[k][r].x - M);
+        for (int k = 0; k < 4; ++k) L += M == -INFINITY ? 0.f : s_ml[k][r].y * ex2(s_ml[k][r].x - M);
         if (whole) {
           const float inv = L > 0.f ? 1.0f / L : 0.f;
           const int tok = r / p.group, hh = r - tok * p.group;
@@ -449,8 +419,9 @@ __global__ void __launch_bounds__(kJThreads) kv_join_kernel(const __grid_constan
       for (int k = c - 1; k <= last; ++k) {
         const int64_t slot = k < c ? first_slot : 2 * static_cast<int64_t>(k);
         const float2 ml = p.part_ml[slot * R + r];
+        if (ml.x == -INFINITY) continue;  // weight 0; its sums were not written
         const float4 b = *reinterpret_cast<const float4*>(p.part_o + (slot * R + r) * 128 + c4);
-        const float w = kv_ex2(ml.x - M);
+        const float w = ex2(ml.x - M);
         L += w * ml.y;
         a.x += w * b.x; a.y += w * b.y; a.z += w * b.z; a.w += w * b.w;
       }
@@ -465,51 +436,6 @@ __global__ void __launch_bounds__(kJThreads) kv_join_kernel(const __grid_constan
 }
 
 // ------------------------------------------------------------------ host
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = [] {
-    void* q = nullptr;
-    cudaDriverEntryPointQueryResult r;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &q, cudaEnableDefault, &r) != cudaSuccess ||
-        r != cudaDriverEntryPointSuccess)
-      q = nullptr;
-    return reinterpret_cast<EncodeTiledFn>(q);
-  }();
-  return fn;
-}
-
-// One cache plane: {channel, token of the block, head, block}, boxes of 64 channels x box_rows tokens.
-cudaError_t cache_map(CUtensorMap* m, const KvCacheView& c, const void* base, int box_rows) {
-  EncodeTiledFn fn = encode_fn();
-  if (!fn) return cudaErrorNotSupported;
-  const cuuint64_t bs = static_cast<cuuint64_t>(c.block_size);
-  cuuint64_t dims[4] = {128, bs, static_cast<cuuint64_t>(c.heads_kv), static_cast<cuuint64_t>(c.n_blocks)};
-  cuuint64_t strides[3] = {256, bs * 256, static_cast<cuuint64_t>(c.block_stride) * 2};
-  cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows), 1, 1};
-  cuuint32_t es[4] = {1, 1, 1, 1};
-  const CUresult r =
-      fn(m, c.f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims,
-         strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
-}
-
-// Dynamic shared memory limit of a kernel, set once per device.
-template <class K>
-cudaError_t allow_smem(K* kernel, int bytes, std::atomic<uint64_t>& done) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  const uint64_t bit = uint64_t(1) << (dev & 63);
-  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
-  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
-  return e;
-}
-
 template <int MT, bool F16>
 cudaError_t launch_rows(const KvCacheView& c, KvAttnArgs a, int grid, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
@@ -517,8 +443,8 @@ cudaError_t launch_rows(const KvCacheView& c, KvAttnArgs a, int grid, cudaStream
   if (e != cudaSuccess) return e;
   a.box_rows = std::min(c.block_size, kRKT);
   CUtensorMap mk, mv;
-  e = cache_map(&mk, c, c.k, a.box_rows);
-  if (e == cudaSuccess) e = cache_map(&mv, c, c.v, a.box_rows);
+  e = kv_cache_map(&mk, c, c.k, a.box_rows);
+  if (e == cudaSuccess) e = kv_cache_map(&mv, c, c.v, a.box_rows);
   if (e != cudaSuccess) return e;
   kv_rows_kernel<MT, F16><<<grid, kRThreads, kRSmem, s>>>(mk, mv, a);
   return cudaGetLastError();
@@ -541,15 +467,72 @@ cudaError_t launch_join(const KvAttnArgs& a, int rows, cudaStream_t s) {
 
 }  // namespace
 
+namespace {
+
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = [] {
+    void* q = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &q, cudaEnableDefault, &r) != cudaSuccess ||
+        r != cudaDriverEntryPointSuccess)
+      q = nullptr;
+    return reinterpret_cast<EncodeTiledFn>(q);
+  }();
+  return fn;
+}
+
+}  // namespace
+
+// One cache plane: {channel, token of the block, head, block}, boxes of 64 channels x box_rows tokens.
+cudaError_t kv_cache_map(CUtensorMap* m, const KvCacheView& c, const void* base, int box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return cudaErrorNotSupported;
+  const cuuint64_t bs = static_cast<cuuint64_t>(c.block_size);
+  cuuint64_t dims[4] = {128, bs, static_cast<cuuint64_t>(c.heads_kv), static_cast<cuuint64_t>(c.n_blocks)};
+  cuuint64_t strides[3] = {256, bs * 256, static_cast<cuuint64_t>(c.block_stride) * 2};
+  cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows), 1, 1};
+  cuuint32_t es[4] = {1, 1, 1, 1};
+  const CUresult r =
+      fn(m, c.f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims,
+         strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+cudaError_t kv_query_map(CUtensorMap* m, const KvAttnArgs& a, bool f16, int box_tokens) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return cudaErrorNotSupported;
+  cuuint64_t dims[3] = {128, static_cast<cuuint64_t>(a.heads), static_cast<cuuint64_t>(a.tokens)};
+  cuuint64_t strides[2] = {256, static_cast<cuuint64_t>(a.ld_q) * 2};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(a.group), static_cast<cuuint32_t>(box_tokens)};
+  cuuint32_t es[3] = {1, 1, 1};
+  const CUresult r =
+      fn(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<uint16_t*>(a.q), dims,
+         strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 KvAttnPlan kv_attention_plan(int heads, int heads_kv, int64_t max_new, int num_sms) {
   const int group = heads / heads_kv;
   KvAttnPlan pl{};
-  pl.unit_rows = max_new * group <= 16 ? 16 : 32;
-  pl.unit_tokens = pl.unit_rows / group;
-  pl.grid = 2 * num_sms;
-  const size_t rows = 2 * static_cast<size_t>(pl.grid) * pl.unit_rows;
-  pl.ml_bytes = rows * sizeof(float2);  // a multiple of 16
-  pl.bytes = pl.ml_bytes + rows * 128 * sizeof(float);
+  const int64_t rows_of_one = max_new * group;
+  if (max_new <= 32 && rows_of_one <= 32) {
+    pl.unit_rows = rows_of_one <= 16 ? 16 : 32;
+    pl.unit_tokens = pl.unit_rows / group;
+    pl.grid = 2 * num_sms;
+  } else {
+    pl.unit_rows = kTcRows;
+    pl.unit_tokens = 2 * (kTcRows / 2 / group);
+    pl.grid = num_sms;
+  }
+  const size_t part_rows = 2 * static_cast<size_t>(pl.grid) * pl.unit_rows;
+  pl.ml_bytes = part_rows * sizeof(float2);  // a multiple of 16
+  pl.bytes = pl.ml_bytes + part_rows * 128 * sizeof(float);
   return pl;
 }
 
@@ -560,6 +543,12 @@ cudaError_t launch_kv_attention(const KvCacheView& c, KvAttnArgs a, const KvAttn
   a.part_ml = static_cast<float2*>(workspace);
   a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan.ml_bytes);
   cudaError_t e;
+  if (plan.unit_rows == kTcRows) {
+    e = launch_kv_tc(c, a, s);
+    if (e != cudaSuccess) return e;
+    return c.f16 ? launch_join<kTcKT, kTcMinTiles, true>(a, plan.unit_rows, s)
+                 : launch_join<kTcKT, kTcMinTiles, false>(a, plan.unit_rows, s);
+  }
   if (plan.unit_rows == 16)
     e = c.f16 ? launch_rows<1, true>(c, a, plan.grid, s) : launch_rows<1, false>(c, a, plan.grid, s);
   else

@@ -13,7 +13,7 @@ namespace dcpp {
 
 constexpr int kKvHeadDim = 128;
 constexpr int kKvMaxPlanBatch = 8192;  // requests of one plan: its prefix sums live in shared memory
-constexpr int kKvMaxGroup = 32;         // query heads per key / value head
+constexpr int kKvMaxGroup = 128;        // query heads per key / value head
 
 // One step's block tables and maps (kv_plan_kernel).
 struct KvPlanArgs {

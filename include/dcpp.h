@@ -299,7 +299,7 @@ dcpp_status dcpp_kv_store(dcpp_ctx* ctx, const dcpp_kv_cache* cache, int64_t tok
  * Block table entries beyond a request's tokens, and what its last block holds
  * behind them, are never used.  Lengths or block ids out of range leave the
  * request's rows undefined and are reported by dcpp_synchronize
- * (DCPP_ERR_INVALID_ARG).  Up to 32 query heads per key / value head. */
+ * (DCPP_ERR_INVALID_ARG).  Up to 128 query heads per key / value head. */
 dcpp_status dcpp_kv_attention_workspace(dcpp_ctx* ctx, const dcpp_kv_cache* cache, int64_t heads, int64_t max_new,
                                         size_t* out_bytes);
 dcpp_status dcpp_kv_attention(dcpp_ctx* ctx, const dcpp_kv_cache* cache, int64_t batch, int64_t tokens, int64_t heads,

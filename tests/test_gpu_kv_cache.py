@@ -235,7 +235,7 @@ def run(ctx, s, causal=True, scale=None):
     s.check(causal, scale)
 
 
-HEADS = [(32, 8), (8, 8), (16, 2), (8, 1), (28, 4), (12, 4), (32, 1)]
+HEADS = [(32, 8), (8, 8), (16, 2), (8, 1), (28, 4), (12, 4), (32, 1), (128, 1)]
 
 
 @pytest.mark.parametrize("heads,heads_kv", HEADS)
