@@ -17,10 +17,6 @@ namespace dcpp {
 
 namespace {
 
-__device__ __forceinline__ void named_sync(int id, int threads) {
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
-
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -387,8 +383,11 @@ __global__ void __launch_bounds__(kRThreads, 2)
 // ------------------------------------------------------------ joining parts
 // Block c looks at the cut between parts c and c + 1.  If it goes through a unit
 // and is the first cut to do so, the block joins that unit's parts, in the order
-// of the parts: the result does not depend on which CTA finished first.
+// of the parts: the result does not depend on which CTA finished first.  A warp
+// per row, 32 rows per block (the y blocks of a cut share the unit's rows): what it
+// costs is latency, a chain of two loads per row.
 constexpr int kJThreads = 256;
+constexpr int kJRows = 32;
 
 template <int KT, int MIN_TILES, bool F16>
 __global__ void __launch_bounds__(kJThreads) kv_join_kernel(const __grid_constant__ KvAttnArgs p, int R) {
@@ -404,34 +403,82 @@ __global__ void __launch_bounds__(kJThreads) kv_join_kernel(const __grid_constan
   const int64_t start = kv_cut(range, c) - at.tile;
   if (kv_cut(range, c - 1) > start) return;  // an earlier cut went through this unit
   const int64_t end = start + at.n_tiles;
-  int last = c;
-  while (last + 1 < range.parts && kv_cut(range, last + 1) < end) ++last;
+  const int last = kv_part_of(range, end - 1);
   const int t0 = at.s.q0 + at.u * p.unit_tokens;
   const int rows = min(p.unit_tokens, at.s.q_len - at.u * p.unit_tokens) * p.group;
-  const int64_t first_slot = 2 * static_cast<int64_t>(c - 1) + 1;
-  for (int r = threadIdx.x >> 5; r < rows; r += kJThreads / 32) {
-    const int c4 = (threadIdx.x & 31) * 4;
-    float M = p.part_ml[first_slot * R + r].x;
-    for (int k = c; k <= last; ++k) M = fmaxf(M, p.part_ml[2 * static_cast<int64_t>(k) * R + r].x);
-    float L = 0.f;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (M != -INFINITY) {
-      for (int k = c - 1; k <= last; ++k) {
-        const int64_t slot = k < c ? first_slot : 2 * static_cast<int64_t>(k);
-        const float2 ml = p.part_ml[slot * R + r];
-        if (ml.x == -INFINITY) continue;  // weight 0; its sums were not written
-        const float4 b = *reinterpret_cast<const float4*>(p.part_o + (slot * R + r) * 128 + c4);
-        const float w = ex2(ml.x - M);
-        L += w * ml.y;
-        a.x += w * b.x; a.y += w * b.y; a.z += w * b.z; a.w += w * b.w;
-      }
+  const int lane = threadIdx.x & 31, c4 = lane * 4;
+  // Part k's slot: the unit starts in part c - 1, goes on in c .. last.
+  auto row_of = [&](int k, int r) {
+    return (2 * static_cast<int64_t>(k) + (k == c - 1 ? 1 : 0)) * R + r;
+  };
+  // A warp's four rows go through the loads together: each is one chain (maxima and
+  // sums, then the parts), and it is the length of a chain that this kernel costs.
+  constexpr int kPer = kJRows / (kJThreads / 32);
+  const int r0 = blockIdx.y * kJRows + (threadIdx.x >> 5) * kPer;
+  if (r0 >= rows) return;
+  float M[kPer], L[kPer];
+  float4 a[kPer];
+#pragma unroll
+  for (int q = 0; q < kPer; ++q) {
+    M[q] = -INFINITY;
+    L[q] = 0.f;
+    a[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  for (int k0 = c - 1; k0 <= last; k0 += 32) {  // lane i holds the maximum and sum of part k0 + i
+    const int n = min(32, last - k0 + 1);
+    float2 ml[kPer];
+    float w[kPer];
+#pragma unroll
+    for (int q = 0; q < kPer; ++q)
+      ml[q] = lane < n && r0 + q < rows ? p.part_ml[row_of(k0 + lane, r0 + q)] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) {
+      float mx = ml[q].x;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      const float Mn = fmaxf(M[q], mx);
+      const float ref = Mn == -INFINITY ? 0.f : Mn;  // no key so far: every weight 0
+      const float keep = ex2(M[q] - ref);
+      w[q] = ex2(ml[q].x - ref);
+      float sum = w[q] * ml[q].y;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      L[q] = L[q] * keep + sum;
+      a[q].x *= keep; a[q].y *= keep; a[q].z *= keep; a[q].w *= keep;
+      M[q] = Mn;
     }
-    const float inv = L > 0.f ? 1.0f / L : 0.f;
+    for (int i = 0; i < n; i += 2) {
+      float4 v[2][kPer];
+      float wi[2][kPer];
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int q = 0; q < kPer; ++q) {
+          wi[e][q] = __shfl_sync(0xffffffffu, w[q], min(i + e, 31));
+          if (i + e >= n) wi[e][q] = 0.f;
+          // A part of weight 0 may not have written its sums.
+          if (wi[e][q] != 0.f) v[e][q] = *reinterpret_cast<const float4*>(p.part_o + row_of(k0 + i + e, r0 + q) * 128 + c4);
+        }
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int q = 0; q < kPer; ++q)
+          if (wi[e][q] != 0.f) {
+            a[q].x = fmaf(wi[e][q], v[e][q].x, a[q].x); a[q].y = fmaf(wi[e][q], v[e][q].y, a[q].y);
+            a[q].z = fmaf(wi[e][q], v[e][q].z, a[q].z); a[q].w = fmaf(wi[e][q], v[e][q].w, a[q].w);
+          }
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < kPer; ++q) {
+    const int r = r0 + q;
+    if (r >= rows) break;
+    const float inv = L[q] > 0.f ? 1.0f / L[q] : 0.f;
     const int tok = r / p.group, hh = r - tok * p.group;
     uint16_t* dst = p.out + static_cast<int64_t>(t0 + tok) * p.ld_out +
                     (static_cast<int64_t>(at.h) * p.group + hh) * 128 + c4;
     *reinterpret_cast<uint2*>(dst) =
-        make_uint2(kv_pack2<F16>(a.x * inv, a.y * inv), kv_pack2<F16>(a.z * inv, a.w * inv));
+        make_uint2(kv_pack2<F16>(a[q].x * inv, a[q].y * inv), kv_pack2<F16>(a[q].z * inv, a[q].w * inv));
   }
 }
 
@@ -453,7 +500,7 @@ cudaError_t launch_rows(const KvCacheView& c, KvAttnArgs a, int grid, cudaStream
 template <int KT, int MIN_TILES, bool F16>
 cudaError_t launch_join(const KvAttnArgs& a, int rows, cudaStream_t s) {
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(a.grid - 1);
+  cfg.gridDim = dim3(a.grid - 1, (rows + kJRows - 1) / kJRows);
   cfg.blockDim = dim3(kJThreads);
   cfg.stream = s;
   cudaLaunchAttribute attr{};
@@ -539,6 +586,9 @@ KvAttnPlan kv_attention_plan(int heads, int heads_kv, int64_t max_new, int num_s
 cudaError_t launch_kv_attention(const KvCacheView& c, KvAttnArgs a, const KvAttnPlan& plan, void* workspace,
                                 cudaStream_t s) {
   a.unit_tokens = plan.unit_tokens;
+  a.unit_shift = -1;
+  for (int i = 0; i <= 8; ++i)
+    if (1 << i == plan.unit_tokens) a.unit_shift = i;
   a.grid = plan.grid;
   a.part_ml = static_cast<float2*>(workspace);
   a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan.ml_bytes);

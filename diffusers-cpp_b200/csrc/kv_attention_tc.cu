@@ -3,21 +3,25 @@
 //
 // A unit is two tiles of up to 128 query rows (tokens x the heads of a key /
 // value group) of one request and key / value head; CTAs (one per SM) walk their
-// run of (unit, key tile) steps.  384 threads:
+// run of (unit, key tile) steps.  352 threads:
 //   warp 0      TMA: Q of a unit, then K_j, V_j (128 keys, gathered block by block)
-//               into a ring of five 32 KB slots
-//   warp 1      TMEM allocation and the MMAs: S_X = Q_X K_j^T, O_X += P_X V_j for
-//               the tiles X = A, B, in the order
-//                 S_A S_B | PV_A S_A' PV_B S_B' | ...
-//   warps 4-7   softmax of tile A, warps 8-11 of tile B: one thread per row
-// The first four warps hand registers to the softmax warps (a row's 128 scores
-// stay in registers): 128 x (96 + 2 x 200) of the 384 x 168 the CTA starts with.
-// V stays as the cache holds it, keys x channels: the P V product reads it as an
-// operand whose rows run along the channels (MN-major), so no transposed copy of
-// the cache is kept.  P goes back over its own scores in TMEM, in two halves of
-// 64 keys, each signalled by itself: the first half's product runs while the
-// second half's exponentials are computed.
-// TMEM (512 columns): S_A / P_A 0, S_B / P_B 128, O_A 256, O_B 384.
+//               into two 64 KB slots
+//   warps 1, 10 the MMAs of tile A and of tile B, one thread each (a wait that is
+//               already met costs some 80 cycles; one thread for both tiles spent
+//               more time in its eight waits per step than the tensor core in its
+//               products)
+//   warps 2-5   softmax of tile A, warps 6-9 of tile B: one thread per row
+// A step is 64 keys.  Scores and numerators have TMEM of their own, so that neither
+// product waits for the other: the scores' buffer is free again as soon as the
+// softmax warps have them in registers, and S(i + 1) is computed while they work on
+// step i; the numerators have two buffers, and P V of step i runs while they work on
+// step i + 1.  (Scores in two buffers with P written back over them, the layout that
+// holds one more step of scores, made S(i + 2) wait for P V(i): a chain of some 2100
+// cycles a step where the softmax needs 1500 and the tensor core 1280.)
+// V stays as the cache holds it, keys x channels: the P V product takes it as an
+// operand whose rows run along the channels (MN-major), so no transposed copy of the
+// cache is kept.
+// TMEM (512 columns): tile X at 128 X: S 0 .. 63, P 64 and 96; O_A 256, O_B 384.
 #include "kv_device.cuh"
 #include "kv_sched.cuh"
 
@@ -27,26 +31,25 @@ namespace dcpp {
 
 namespace {
 
-constexpr int kTThreads = 384;
-constexpr int kTSlots = 5;
+constexpr int kTThreads = 352;
+constexpr int kTSlots = 2;                // tiles of K and V in flight
 constexpr int kTHalf = 128 * 128;         // 128 rows x 64 channels: 16 KB
 constexpr int kTTile = 2 * kTHalf;        // 128 x 128: 32 KB
-constexpr int kTSmem = (2 + kTSlots) * kTTile + 1024;
+constexpr int kTSmem = (2 + 2 * kTSlots) * kTTile + 1024;
 constexpr float kTRescale = 8.0f;         // log2 units a row maximum may grow before O is rescaled
 
 struct TcBars {
-  uint64_t q_full, q_empty;
-  uint64_t full[kTSlots], empty[kTSlots];
-  uint64_t s_full[2];
-  uint64_t p_full[2][2];  // [tile][half], 128 arrivals
-  uint64_t pv_done[2];
+  uint64_t q_full, q_empty;                // empty barriers: one arrival from each MMA thread
+  uint64_t full[2][kTSlots], empty[2][kTSlots];  // [K, V][slot]
+  uint64_t s_full[2], s_free[2];           // [tile] scores computed; read (4 warps)
+  uint64_t p_full[2][2], pv_done[2][2];    // [tile][buffer] P written (4 warps); P read, O current
 };
 
-// Instruction descriptor: M 128, N 128, f32 accumulator, both operands of the
+// Instruction descriptor: M 128, N columns, f32 accumulator, both operands of the
 // cache's type; B_MN: the B operand's rows run along N.
-template <bool F16, bool B_MN>
+template <bool F16, int N, bool B_MN>
 __host__ __device__ constexpr uint32_t tc_idesc() {
-  return (1u << 4) | (F16 ? 0u : (1u << 7) | (1u << 10)) | (B_MN ? 1u << 16 : 0u) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+  return (1u << 4) | (F16 ? 0u : (1u << 7) | (1u << 10)) | (B_MN ? 1u << 16 : 0u) | (static_cast<uint32_t>(N >> 3) << 17) | ((128u >> 4) << 24);
 }
 
 // Descriptor of a 128-byte-swizzled operand whose rows (64 channels each) run
@@ -61,11 +64,44 @@ __device__ __forceinline__ uint64_t tc_desc_mn(uint32_t addr) {
   return d;
 }
 
-// What a CTA does with the unit at `at`: its key tiles [first, last), and of those
-// the ones that each row tile needs (a causal tile A ends before tile B).
+// The MMA warps' instructions, issued by the one lane whose `leader` is set; barriers
+// by their shared-memory address.
+__device__ __forceinline__ void tc_mma_ss(uint32_t leader, uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc,
+                                          uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void tc_mma_ts(uint32_t leader, uint32_t d, uint32_t a, uint32_t b_lo, uint32_t hi, uint32_t idesc,
+                                          uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void tc_commit(uint32_t leader, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+      "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ bool tc_wait(uint32_t bar, uint32_t phase, int* err) {
+  return kv_wait_warp(bar, phase & 1, err);
+}
+
+// What a CTA does with the unit at `at`: its key tiles [first, last), and the steps
+// of 64 keys, from 2 first on, that each row tile needs of them.
 struct TcWork {
   int first, last;
-  int end[2];
+  int end[2];  // in steps of 64 keys
   int tok0, n_tok[2];  // first token of the unit, tokens of each tile
 };
 
@@ -81,15 +117,44 @@ __device__ __forceinline__ TcWork tc_work(const KvAttnArgs& p, const KvPos& at, 
     w.n_tok[x] = min(max(n - x * half, 0), half);
     int keys = at.s.kv;
     if (p.causal) keys = min(keys, at.s.off + w.tok0 + x * half + w.n_tok[x]);
-    const int tiles = w.n_tok[x] > 0 ? max(1, (keys + kTcKT - 1) / kTcKT) : 0;
-    w.end[x] = max(w.first, min(w.last, tiles));
+    const int steps = w.n_tok[x] > 0 ? max(1, (keys + 63) >> 6) : 0;
+    w.end[x] = max(2 * w.first, min(2 * w.last, steps));
   }
   return w;
+}
+
+// Eight f32 values times `by`, rounded to the output's type.
+template <bool F16>
+__device__ __forceinline__ uint4 tc_pack8(const uint32_t* r, float by) {
+  return make_uint4(kv_pack2<F16>(__uint_as_float(r[0]) * by, __uint_as_float(r[1]) * by),
+                    kv_pack2<F16>(__uint_as_float(r[2]) * by, __uint_as_float(r[3]) * by),
+                    kv_pack2<F16>(__uint_as_float(r[4]) * by, __uint_as_float(r[5]) * by),
+                    kv_pack2<F16>(__uint_as_float(r[6]) * by, __uint_as_float(r[7]) * by));
+}
+
+// Among eight lanes: lane i's piece k goes to lane k's place i.
+__device__ __forceinline__ void tc_trade8(uint4 (&v)[8], int lane) {
+#pragma unroll
+  for (int s = 1; s < 8; s <<= 1) {
+    const bool up = lane & s;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (k & s) continue;
+      const uint4 give = up ? v[k] : v[k | s];
+      uint4 got;
+      got.x = __shfl_xor_sync(0xffffffffu, give.x, s);
+      got.y = __shfl_xor_sync(0xffffffffu, give.y, s);
+      got.z = __shfl_xor_sync(0xffffffffu, give.z, s);
+      got.w = __shfl_xor_sync(0xffffffffu, give.w, s);
+      if (up) v[k] = got; else v[k | s] = got;
+    }
+  }
 }
 
 struct TcState {
   KvPos at;
   int64_t left;
+  int tiles;  // key tiles of the runs before this one
 };
 
 template <bool F16>
@@ -108,16 +173,19 @@ __global__ void __launch_bounds__(kTThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     mbar_init(&bar.q_full, 1);
-    mbar_init(&bar.q_empty, 1);
-    for (int i = 0; i < kTSlots; ++i) {
-      mbar_init(&bar.full[i], 1);
-      mbar_init(&bar.empty[i], 1);
-    }
+    mbar_init(&bar.q_empty, 2);
+    for (int i = 0; i < kTSlots; ++i)
+      for (int kv = 0; kv < 2; ++kv) {
+        mbar_init(&bar.full[kv][i], 1);
+        mbar_init(&bar.empty[kv][i], 2);
+      }
     for (int x = 0; x < 2; ++x) {
       mbar_init(&bar.s_full[x], 1);
-      mbar_init(&bar.p_full[x][0], 128);
-      mbar_init(&bar.p_full[x][1], 128);
-      mbar_init(&bar.pv_done[x], 1);
+      mbar_init(&bar.s_free[x], 4);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&bar.p_full[x][b], 4);
+        mbar_init(&bar.pv_done[x][b], 1);
+      }
     }
     fence_barrier_init();
     tma_prefetch_desc(&tmQ);
@@ -141,18 +209,17 @@ __global__ void __launch_bounds__(kTThreads, 1)
   int64_t left = have ? kv_cut(range, blockIdx.x + 1) - kv_cut(range, blockIdx.x) : 0;
   const int half_tok = p.unit_tokens / 2;
 
-  if (warp < 4) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
   if (warp == 0) {
     const int boxes = kTcKT / p.box_rows;
     const int box = lane & (boxes - 1), half = lane / boxes;
     const int bs_mask = (1 << p.block_shift) - 1;
     const uint32_t q_bytes = 2u * 128u * static_cast<uint32_t>(half_tok * p.group);
-    int it = 0, unit = 0;
+    int it = 0, unit = 0;          // key tiles and units so far
+    int issued[2] = {0, 0};        // copies of K and of V
     bool ok = true;
     while (left > 0 && ok) {
       const TcWork w = tc_work(p, at, left);
-      ok = __all_sync(0xffffffffu, kv_wait(&bar.q_empty, (unit & 1) ^ 1, p.err));
+      ok = kv_wait_warp(&bar.q_empty, (unit & 1) ^ 1, p.err);
       if (!ok) break;
       if (lane == 0) {
         mbar_arrive_expect_tx(&bar.q_full, w.n_tok[1] > 0 ? 2 * q_bytes : q_bytes);
@@ -183,142 +250,149 @@ __global__ void __launch_bounds__(kTThreads, 1)
         if (load && wrong) record_error(p.err, kDevBadCache);
         const int c3 = wrong ? p.n_blocks : blk;  // one past the end: TMA fills zeros
         const int loads = __popc(__ballot_sync(0xffffffffu, load));
-        for (int kv = 0; kv < 2; ++kv, ++it) {  // K_j, then V_j
-          const int st = it % kTSlots;
-          ok = __all_sync(0xffffffffu, kv_wait(&bar.empty[st], ((it / kTSlots) & 1) ^ 1, p.err));
+        const int st = it & 1;
+        for (int kv = 0; kv < 2 && ok; ++kv) {  // K_j, then V_j
+          ok = kv_wait_warp(&bar.empty[kv][st], ((it >> 1) & 1) ^ 1, p.err);
           if (!ok) break;
-          if (lane == 0) mbar_arrive_expect_tx(&bar.full[st], loads * p.box_rows * 128);
+          if (lane == 0) mbar_arrive_expect_tx(&bar.full[kv][st], loads * p.box_rows * 128);
           __syncwarp();
           if (load)
-            tma_load_4d(sKV + st * kTTile + half * kTHalf + box * p.box_rows * 128, kv ? &tmV : &tmK, &bar.full[st],
-                        half * 64, key0 & bs_mask, at.h, c3);
+            tma_load_4d(sKV + (2 * st + kv) * kTTile + half * kTHalf + box * p.box_rows * 128, kv ? &tmV : &tmK,
+                        &bar.full[kv][st], half * 64, key0 & bs_mask, at.h, c3);
+          issued[kv] = it + 1;
         }
+        ++it;
       }
       left -= w.last - w.first;
       if (left > 0 && !kv_next_unit<kTcKT>(p, at)) break;
     }
     // Nothing may be in flight when the CTA ends: all copies landed, and (unless a
     // wait ran out) every slot handed back, i.e. the last commits have arrived.
-    for (int k = max(0, it - kTSlots); k < it; ++k)
-      if (!kv_wait(&bar.full[k % kTSlots], (k / kTSlots) & 1, p.err)) ok = false;
-    if (unit > 0 && !kv_wait(&bar.q_full, (unit - 1) & 1, p.err)) ok = false;
-    if (ok) {
-      for (int k = max(0, it - kTSlots); k < it; ++k)
-        if (!kv_wait(&bar.empty[k % kTSlots], (k / kTSlots) & 1, p.err)) break;
-      if (unit > 0) kv_wait(&bar.q_empty, (unit - 1) & 1, p.err);
+    bool landed = unit == 0 || kv_wait(&bar.q_full, (unit - 1) & 1, p.err);
+    for (int kv = 0; kv < 2; ++kv)
+      for (int k = max(0, issued[kv] - kTSlots); k < issued[kv]; ++k)
+        landed &= kv_wait(&bar.full[kv][k & 1], (k >> 1) & 1, p.err);
+    if (ok && landed && unit > 0) {
+      for (int kv = 0; kv < 2; ++kv)
+        for (int k = max(0, it - kTSlots); k < it; ++k) ok = ok && kv_wait(&bar.empty[kv][k & 1], (k >> 1) & 1, p.err);
+      if (ok) kv_wait(&bar.q_empty, (unit - 1) & 1, p.err);
     }
-  } else if (warp == 1) {
-    // The whole warp runs the loop; one elected lane issues the MMAs and commits.
-    constexpr uint32_t idS = tc_idesc<F16, false>(), idPV = tc_idesc<F16, true>();
-    const uint64_t dQ = make_sdesc_sw128(smem_u32(sQ));
+  } else if (warp == 1 || warp == kTThreads / 32 - 1) {
+    // The whole warp runs the loop, without a branch around the products: one elected
+    // lane issues them by predicate.
+    const int x = warp == 1 ? 0 : 1;
+    constexpr uint32_t idS = tc_idesc<F16, 64, false>(), idPV = tc_idesc<F16, 128, true>();
+    const uint64_t dQ = make_sdesc_sw128(smem_u32(sQ + x * kTTile));
     const uint64_t dK = make_sdesc_sw128(smem_u32(sKV));
-    const uint64_t dV = tc_desc_mn(smem_u32(sKV));
-    auto koff = [](int k) -> uint64_t { return static_cast<uint64_t>(((k >> 2) * kTHalf + (k & 3) * 32) >> 4); };
-    constexpr uint64_t kTileD = kTTile >> 4;
-    const bool leader = elect_one_sync();
-    int it = 0, unit = 0;
-    int n_pv[2] = {0, 0}, n_p[2] = {0, 0};
+    const uint64_t dV = tc_desc_mn(smem_u32(sKV + kTTile));
+    // The descriptors' low words; a slot, a step or a K step only moves the address in them.
+    const uint32_t hiK = static_cast<uint32_t>(dK >> 32), hiV = static_cast<uint32_t>(dV >> 32);
+    const uint32_t loQ = static_cast<uint32_t>(dQ), loK = static_cast<uint32_t>(dK), loV = static_cast<uint32_t>(dV);
+    constexpr uint32_t kSlotD = 2 * kTTile >> 4, kStepD = 64 * 128 >> 4;
+    const uint32_t tS = tmem + x * 128, tO = tmem + 256 + x * 128;
+    const uint32_t fullK = smem_u32(bar.full[0]), fullV = smem_u32(bar.full[1]);
+    const uint32_t emptyK = smem_u32(bar.empty[0]), emptyV = smem_u32(bar.empty[1]);
+    const uint32_t s_full = smem_u32(&bar.s_full[x]), s_free = smem_u32(&bar.s_free[x]);
+    const uint32_t p_full = smem_u32(bar.p_full[x]), pv_done = smem_u32(bar.pv_done[x]), q_empty = smem_u32(&bar.q_empty);
+    const uint32_t leader = elect_one_sync();
+    int unit = 0, n = 0, n_s = 0;  // units; P V products and scores issued for this tile
+    int tk = 0, tv = 0;            // tiles whose K, and whose V, this warp is done with
     bool ok = true;
-    auto wait = [&](uint64_t* b, int phase) {
-      ok = __all_sync(0xffffffffu, ok && kv_wait(b, phase & 1, p.err));
-      if (ok) tc_fence_after();
-      return ok;
-    };
-    // S_X = Q_X K^T from slot `slot`; last: the last use of this K slot; done: of this unit's Q.
-    auto issue_s = [&](int x, int slot, bool last, bool done) {
-      if (n_pv[x] > 0 && !wait(&bar.pv_done[x], n_pv[x] - 1)) return;  // P over S has been read
-      if (leader) {
-        const uint64_t q = dQ + x * kTileD, kd = dK + slot * kTileD;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) umma_bf16(tmem + x * 128, q + koff(k), kd + koff(k), idS, k > 0 ? 1u : 0u);
-        umma_commit(&bar.s_full[x]);
-        if (last) umma_commit(&bar.empty[slot]);
-        if (done) umma_commit(&bar.q_empty);
-      }
-      __syncwarp();
-    };
     while (left > 0 && ok) {
       const TcWork w = tc_work(p, at, left);
-      const int top = w.n_tok[1] > 0 ? 1 : 0;  // the tile that needs every key tile of the run
-      if (!wait(&bar.q_full, unit)) break;
-      ++unit;
-      const int n = w.last - w.first;
-      auto k_slot = [&](int i) { return (it + 2 * i) % kTSlots; };
-      auto k_phase = [&](int i) { return (it + 2 * i) / kTSlots; };
-      if (!wait(&bar.full[k_slot(0)], k_phase(0))) break;
-      for (int x = 0; x <= top && ok; ++x)
-        if (w.first < w.end[x]) issue_s(x, k_slot(0), x == top, x == top && n == 1);
-      for (int i = 0; i < n && ok; ++i) {
-        const int j = w.first + i;
-        const int vs = (it + 2 * i + 1) % kTSlots;
-        if (!wait(&bar.full[vs], (it + 2 * i + 1) / kTSlots)) break;
-        const int valid = at.s.kv - j * kTcKT;
-        if (valid < kTcKT) {
-          // Behind the last key a block holds anything, and 0 x NaN is NaN: clear those rows.
-          uint8_t* v = sKV + vs * kTTile;
-          for (int c = max(valid, 0) * 8 + lane; c < kTcKT * 8; c += 32) {
-            *reinterpret_cast<uint4*>(v + c * 16) = make_uint4(0, 0, 0, 0);
-            *reinterpret_cast<uint4*>(v + kTHalf + c * 16) = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-        }
-        for (int x = 0; x <= top && ok; ++x) {
-          if (j >= w.end[x]) continue;
-          const uint32_t tO = tmem + 256 + x * 128, tP = tmem + x * 128;
-          const uint64_t vd = dV + vs * kTileD;
-          for (int h = 0; h < 2; ++h) {
-            if (!wait(&bar.p_full[x][h], n_p[x])) break;
-            if (leader) {
+      const int s0 = 2 * w.first, end = w.end[x], tiles = w.last - w.first;
+      const bool twice = w.n_tok[1] == 0;  // without a tile B, tile A's warp arrives for both
+      // Both warps meet every phase of the barriers in order, used or not: a parity
+      // wait tells a phase only from its neighbours.
+      if (!(ok = kv_wait_warp(&bar.q_full, unit & 1, p.err))) break;
+      // Hands back a slot (or Q) once the MMAs issued so far are done.
+      auto release = [&](uint32_t b) {
+        tc_commit(leader, b);
+        if (twice) tc_commit(leader, b);
+      };
+      if (x == 1 && twice) {
+        for (int k = 0; k < tiles && ok; ++k, ++tk, ++tv)
+          ok = tc_wait(fullK + 8 * (tk & 1), tk >> 1, p.err) && tc_wait(fullV + 8 * (tv & 1), tv >> 1, p.err);
+      } else {
+        if (end == s0) release(q_empty);
+        // S(i + 1) = Q K_{i+1}^T, then O += P(i) V_i.
+#pragma unroll 1
+        for (int i = s0 - 1; i < end; ++i) {
+          const int is = i + 1;
+          if (is < end) {
+            if (!(is & 1) && !(ok = tc_wait(fullK + 8 * (tk & 1), tk >> 1, p.err))) break;
+            if (n_s > 0 && !(ok = tc_wait(s_free, n_s - 1, p.err))) break;
+            tc_fence_after();
+            const uint32_t kd = loK + (tk & 1) * kSlotD + (is & 1) * kStepD;
 #pragma unroll
-              for (int k = 0; k < 4; ++k)  // 16 keys: 8 packed TMEM columns of P, 16 rows (2 KB) of V
-                umma_bf16_ts(tO, tP + h * 32 + k * 8, vd + ((h * 4 + k) * 2048 >> 4), idPV, i > 0 || h > 0 || k > 0 ? 1u : 0u);
-              if (h == 1) {
-                umma_commit(&bar.pv_done[x]);
-                if (x == top) umma_commit(&bar.empty[vs]);
-              }
+            for (int k = 0; k < 8; ++k) {
+              const uint32_t off = ((k >> 2) * kTHalf + (k & 3) * 32) >> 4;
+              tc_mma_ss(leader, tS, loQ + off, kd + off, hiK, idS, k > 0);
             }
-            __syncwarp();
+            tc_commit(leader, s_full);
+            if ((is & 1) || is + 1 == end) {
+              release(emptyK + 8 * (tk & 1));
+              ++tk;
+              if (is + 1 == end) release(q_empty);
+            }
+            ++n_s;
           }
-          if (!ok) break;
-          ++n_p[x];
-          ++n_pv[x];
-          if (j + 1 < w.end[x]) {
-            if (!wait(&bar.full[k_slot(i + 1)], k_phase(i + 1))) break;
-            issue_s(x, k_slot(i + 1), x == top, x == top && i + 2 == n);
+          if (i >= s0) {
+            const uint32_t b = n & 1;
+            if ((!(i & 1) || i == s0) && !(ok = tc_wait(fullV + 8 * (tv & 1), tv >> 1, p.err))) break;
+            if (!(ok = tc_wait(p_full + 8 * b, n >> 1, p.err))) break;
+            tc_fence_after();
+            const uint32_t tP = tS + 64 + b * 32, vd = loV + (tv & 1) * kSlotD + (i & 1) * kStepD;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)  // 16 keys: 8 packed TMEM columns of P, 16 rows (2 KB) of V
+              tc_mma_ts(leader, tO, tP + k * 8, vd + k * (2048 >> 4), hiV, idPV, i > s0 || k > 0);
+            tc_commit(leader, pv_done + 8 * b);
+            if ((i & 1) || i + 1 == end) {
+              release(emptyV + 8 * (tv & 1));
+              ++tv;
+            }
+            ++n;
           }
+        }
+        // Tiles of the run that only the other row tile needs.
+        for (int j = (end + 1) >> 1; j < w.last && ok; ++j, ++tk, ++tv) {
+          if (!(ok = tc_wait(fullK + 8 * (tk & 1), tk >> 1, p.err) && tc_wait(fullV + 8 * (tv & 1), tv >> 1, p.err))) break;
+          release(emptyK + 8 * (tk & 1));
+          release(emptyV + 8 * (tv & 1));
         }
       }
-      it += 2 * n;
-      left -= n;
+      ++unit;
+      left -= tiles;
       if (left > 0 && !kv_next_unit<kTcKT>(p, at)) break;
     }
-  }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-    const int x = (warp - 4) >> 2;
+    const int x = (warp - 2) >> 2;
     const int row = (warp & 3) * 32 + lane;  // TMEM lane
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + lane_off + x * 128, tO = tmem + lane_off + 256 + x * 128;
+    const uint32_t s_full = smem_u32(&bar.s_full[x]), s_free = smem_u32(&bar.s_free[x]);
+    const uint32_t p_full = smem_u32(bar.p_full[x]), pv_done = smem_u32(bar.pv_done[x]);
     const float c = p.scale_log2;
-    int n_s = 0;
+    int n = 0;  // steps done by this tile
     bool ok = true;
     // The walk's state rests in shared memory while a unit is computed: its registers
     // are needed for the scores.
-    TcState& st = state[warp - 4];
+    TcState& st = state[warp - 2];
     if (lane == 0) {
       st.at = at;
       st.left = left;
+      st.tiles = 0;
     }
     __syncwarp();
     while (ok && st.left > 0) {
-      int first, end, limit, all_below;
+      int first, end, keys, limit, all_below;
       {
         const KvPos u = st.at;
         const TcWork w = tc_work(p, u, st.left);
-        first = w.first;
+        first = 2 * w.first;
         end = w.end[x];
         const int tile0 = u.s.off + w.tok0 + x * half_tok;  // position of the tile's first token
+        keys = u.s.kv;
         limit = u.s.kv;  // keys this row attends to: [0, limit)
         if (p.causal) limit = min(limit, tile0 + row / p.group + 1);
         all_below = u.s.kv;  // keys that every row of the tile attends to
@@ -326,77 +400,91 @@ __global__ void __launch_bounds__(kTThreads, 1)
       }
       float m = -INFINITY, l = 0.f;
 #pragma unroll 1
-      for (int j = first; j < end; ++j) {
-        ok = __all_sync(0xffffffffu, kv_wait(&bar.s_full[x], n_s & 1, p.err));
-        if (!ok) break;
-        ++n_s;
+      for (int i = first; i < end; ++i, ++n) {
+        const int b = n & 1;
+        if (!(ok = kv_wait_warp(s_full, n & 1, p.err))) break;
         tc_fence_after();
-        float s[128];
+        float s[64];
         {
-          uint32_t r0[32], r1[32], r2[32], r3[32];
+          uint32_t r0[32], r1[32];
           tmem_ld32(tS, r0);
           tmem_ld32(tS + 32, r1);
-          tmem_ld32(tS + 64, r2);
-          tmem_ld32(tS + 96, r3);
           tmem_ld_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_at(s_free);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            s[i] = __uint_as_float(r0[i]);
-            s[32 + i] = __uint_as_float(r1[i]);
-            s[64 + i] = __uint_as_float(r2[i]);
-            s[96 + i] = __uint_as_float(r3[i]);
+          for (int k = 0; k < 32; ++k) {
+            s[k] = __uint_as_float(r0[k]);
+            s[32 + k] = __uint_as_float(r1[k]);
           }
         }
-        const int kbase = j * kTcKT;
-        if (kbase + kTcKT > all_below) {
+        const int kbase = i * 64;
+        if (kbase + 64 > all_below) {
+          if (kbase + 64 > keys) {
+            // Behind the last key a block holds anything, and 0 x NaN is NaN: clear those
+            // rows of V (both row tiles do; zeros over zeros).
+            const int tile = st.tiles + (i >> 1) - (first >> 1);
+            if (!(ok = kv_wait_warp(&bar.full[1][tile & 1], (tile >> 1) & 1, p.err))) break;
+            uint8_t* v = sKV + (2 * (tile & 1) + 1) * kTTile + (i & 1) * 64 * 128;
+#pragma unroll 1
+            for (int k = max(keys - kbase, 0) * 8 + row; k < 64 * 8; k += 128) {
+              *reinterpret_cast<uint4*>(v + k * 16) = make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4*>(v + kTHalf + k * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+          }
 #pragma unroll
-          for (int i = 0; i < 128; ++i)
-            if (kbase + i >= limit) s[i] = -INFINITY;
+          for (int k = 0; k < 64; ++k)
+            if (kbase + k >= limit) s[k] = -INFINITY;
         }
-        float mp[8];
+        float mp[4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) mp[k] = s[k];
+        for (int k = 0; k < 4; ++k) mp[k] = s[k];
 #pragma unroll
-        for (int i = 8; i < 128; i += 2) mp[(i >> 1) & 7] = max3(mp[(i >> 1) & 7], s[i], s[i + 1]);
-        const float mx = c * max3(max3(mp[0], mp[1], mp[2]), max3(mp[3], mp[4], mp[5]), fmaxf(mp[6], mp[7]));
+        for (int k = 4; k < 64; k += 2) mp[(k >> 1) & 3] = max3(mp[(k >> 1) & 3], s[k], s[k + 1]);
+        const float mx = c * fmaxf(max3(mp[0], mp[1], mp[2]), mp[3]);
         const bool grow = mx > m + kTRescale;
         const float m_use = grow ? mx : m;
         // A stale maximum is exact (l uses the same one); without a key so far every numerator is 0.
         const float ref = m_use == -INFINITY ? 0.f : m_use;
         const float alpha = grow ? ex2(m - ref) : 1.0f;
+        if (i > first && __any_sync(0xffffffffu, grow)) {
+          // O has to hold every earlier step before it is rescaled.
+          if (!(ok = kv_wait_warp(pv_done + 8 * (b ^ 1), ((n - 1) >> 1) & 1, p.err))) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int ch = 0; ch < 8; ++ch) {
+            uint32_t r[16];
+            tmem_ld16(tO + ch * 16, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int k = 0; k < 16; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * alpha);
+            tmem_st16(tO + ch * 16, r);
+          }
+        }
         const uint64_t c2 = f2(c, c), nm2 = f2(-ref, -ref);
         uint64_t sp[4] = {0, 0, 0, 0};
+        uint32_t pk[32];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t pk[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const uint64_t y = fma2(f2(s[h * 64 + 2 * i], s[h * 64 + 2 * i + 1]), c2, nm2);
-            const uint64_t e = (i & 3) == 3 ? ex2_poly2(y) : f2(ex2(f2lo(y)), ex2(f2hi(y)));
-            sp[i & 3] = add2(sp[i & 3], e);
-            pk[i] = kv_pack2<F16>(f2lo(e), f2hi(e));
-          }
-          if (h == 0 && j > first && __any_sync(0xffffffffu, grow)) {  // S_j complete: so is P V of every earlier tile
-#pragma unroll 1
-            for (int ch = 0; ch < 4; ++ch) {
-              uint32_t r[32];
-              tmem_ld32(tO + ch * 32, r);
-              tmem_ld_wait();
-#pragma unroll
-              for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
-              tmem_st32(tO + ch * 32, r);
-            }
-          }
-          tmem_st32(tS + h * 32, pk);
-          tmem_st_wait();
-          tc_fence_before();
-          mbar_arrive(&bar.p_full[x][h]);
+        for (int k = 0; k < 32; ++k) {
+          const uint64_t y = fma2(f2(s[2 * k], s[2 * k + 1]), c2, nm2);
+          const uint64_t e = (k & 3) == 3 ? ex2_poly2(y) : f2(ex2(f2lo(y)), ex2(f2hi(y)));
+          sp[k & 3] = add2(sp[k & 3], e);
+          pk[k] = kv_pack2<F16>(f2lo(e), f2hi(e));
+          // P V of step n - 2, which read this buffer, was issued before the scores of step n.
+          if (k == 15) tmem_st16(tS + 64 + b * 32, pk);
         }
+        tmem_st16(tS + 80 + b * 32, pk + 16);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_at(p_full + 8 * b);
         const uint64_t t = add2(add2(sp[0], sp[1]), add2(sp[2], sp[3]));
         l = l * alpha + f2lo(t) + f2hi(t);
         m = m_use;
       }
-      if (ok && first < end) ok = __all_sync(0xffffffffu, kv_wait(&bar.pv_done[x], (n_s - 1) & 1, p.err));
+      if (ok && first < end) ok = kv_wait_warp(pv_done + 8 * ((n - 1) & 1), ((n - 1) >> 1) & 1, p.err);
       if (!ok) break;
       const KvPos u = st.at;
       const TcWork w = tc_work(p, u, st.left);
@@ -404,52 +492,63 @@ __global__ void __launch_bounds__(kTThreads, 1)
       const int tok = w.tok0 + x * half_tok + tok_in;
       const bool mine = tok_in < w.n_tok[x];
       const bool whole = w.first == 0 && w.last == u.n_tiles;
-      uint32_t r0[32], r1[32], r2[32], r3[32];
-      tc_fence_after();
-      tmem_ld32(tO, r0);
-      tmem_ld32(tO + 32, r1);
-      tmem_ld32(tO + 64, r2);
-      tmem_ld32(tO + 96, r3);
-      tmem_ld_wait();
-      tc_fence_before();
-      const uint32_t* rs[4] = {r0, r1, r2, r3};
+      // A lane holds a row; a store of one row per lane would touch 32 lines with 16
+      // bytes each.  So eight lanes trade 16-byte pieces until each holds the same
+      // piece of all eight rows, and write 128 bytes of a row together.
+      uint8_t* dst = nullptr;
       if (mine && whole) {
-        const float inv = m != -INFINITY ? 1.0f / l : 0.f;
-        uint16_t* dst = p.out + static_cast<int64_t>(u.s.q0 + tok) * p.ld_out +
-                        (static_cast<int64_t>(u.h) * p.group + head_in) * 128;
-#pragma unroll
-        for (int ch = 0; ch < 4; ++ch) {
-          uint4* d4 = reinterpret_cast<uint4*>(dst + ch * 32);
-          const uint32_t* r = rs[ch];
-#pragma unroll
-          for (int v = 0; v < 4; ++v)
-            d4[v] = make_uint4(
-                kv_pack2<F16>(__uint_as_float(r[8 * v]) * inv, __uint_as_float(r[8 * v + 1]) * inv),
-                kv_pack2<F16>(__uint_as_float(r[8 * v + 2]) * inv, __uint_as_float(r[8 * v + 3]) * inv),
-                kv_pack2<F16>(__uint_as_float(r[8 * v + 4]) * inv, __uint_as_float(r[8 * v + 5]) * inv),
-                kv_pack2<F16>(__uint_as_float(r[8 * v + 6]) * inv, __uint_as_float(r[8 * v + 7]) * inv));
-        }
+        dst = reinterpret_cast<uint8_t*>(p.out + static_cast<int64_t>(u.s.q0 + tok) * p.ld_out +
+                                         (static_cast<int64_t>(u.h) * p.group + head_in) * 128);
       } else if (mine) {
         const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (w.first == 0 ? 1 : 0);
         // Rows of a unit in order of (token, head): tile B follows tile A's half_tok * group rows.
         const int64_t at_row = slot * kTcRows + x * half_tok * p.group + row;
         p.part_ml[at_row] = make_float2(m, m != -INFINITY ? l : 0.f);
-        if (m != -INFINITY) {  // a part of weight 0 is never read
-          float4* d4 = reinterpret_cast<float4*>(p.part_o + at_row * 128);
-#pragma unroll
-          for (int ch = 0; ch < 4; ++ch)
-#pragma unroll
-            for (int v = 0; v < 8; ++v)
-              d4[ch * 8 + v] = make_float4(__uint_as_float(rs[ch][4 * v]), __uint_as_float(rs[ch][4 * v + 1]),
-                                           __uint_as_float(rs[ch][4 * v + 2]), __uint_as_float(rs[ch][4 * v + 3]));
-        }
+        if (m != -INFINITY) dst = reinterpret_cast<uint8_t*>(p.part_o + at_row * 128);  // a part of weight 0 is never read
       }
+      uint8_t* to[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        to[k] = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), (lane & 24) + k));
+      tc_fence_after();
+      const float inv = m != -INFINITY ? 1.0f / l : 0.f;
+#pragma unroll 1
+      for (int g = 0; g < 4; ++g) {  // 32 columns at a time; two of them make a piece of 128 bytes of output
+        uint4 v[8];
+        int at_byte = g * 128;
+        {
+          uint32_t r[32];
+          tmem_ld32(tO + g * 32, r);
+          tmem_ld_wait();
+          if (whole) {
+            uint32_t q[32];
+            tmem_ld32(tO + g * 32 + 32, q);
+            tmem_ld_wait();
+            at_byte = g * 64;
+            ++g;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              v[k] = tc_pack8<F16>(r + k * 8, inv);
+              v[4 + k] = tc_pack8<F16>(q + k * 8, inv);
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
+          }
+        }
+        tc_trade8(v, lane);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (to[k]) *reinterpret_cast<uint4*>(to[k] + at_byte + (lane & 7) * 16) = v[k];
+      }
+      tc_fence_before();
       __syncwarp();
       if (lane == 0) {
         KvPos next = st.at;
         const int64_t rest = st.left - (w.last - w.first);
         st.left = rest > 0 && kv_next_unit<kTcKT>(p, next) ? rest : 0;
         st.at = next;
+        st.tiles += w.last - w.first;
       }
       __syncwarp();
     }

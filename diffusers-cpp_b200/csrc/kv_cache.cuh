@@ -73,6 +73,7 @@ struct KvAttnArgs {
   int32_t causal;
   float scale_log2;         // scale * log2(e)
   int32_t unit_tokens;      // query tokens of one work unit
+  int32_t unit_shift;       // log2 of it, -1: not a power of two
   int32_t grid;             // CTAs of the main kernel
   float* part_o;            // [2 * grid][unit rows][128] partial sums
   float2* part_ml;          // [2 * grid][unit rows] their running maximum and sum

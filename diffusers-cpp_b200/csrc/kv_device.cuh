@@ -19,18 +19,69 @@ __device__ __forceinline__ uint32_t kv_pack2(float lo, float hi) {
   }
 }
 
+// One try on the barrier at a shared-memory address (the thread may sleep for a while in it).
+__device__ __forceinline__ bool kv_try_wait(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+
+__device__ __forceinline__ void mbar_arrive_at(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
 // Bounded wait that looks at nothing but its barrier and the clock: another
-// kernel's recorded error does not end this one's work.
-__device__ __forceinline__ bool kv_wait(uint64_t* bar, uint32_t parity, int* err) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const unsigned long long t0 = globaltimer();
-  for (;;) {
-    if (mbar_try_wait_sleep(bar, parity, 20000u)) return true;
-    if (globaltimer() - t0 > kWaitTimeoutNs) {
-      record_error(err, kDevTimeoutKv);
-      return false;
+// kernel's recorded error does not end this one's work.  The part behind the first
+// try stays out of line: these kernels' loops are long, and instruction fetch counts.
+static __device__ __noinline__ bool kv_wait_on(uint32_t bar, uint32_t parity, int* err) {
+  unsigned long long t0 = 0;
+  for (uint32_t k = 1;; ++k) {
+    if (kv_try_wait(bar, parity)) return true;
+    if ((k & 255u) == 0) {  // the clock is slow to read: not on the way of a wait that ends soon
+      const unsigned long long t = globaltimer();
+      if (t0 == 0) t0 = t;
+      if (t - t0 > kWaitTimeoutNs) {
+        record_error(err, kDevTimeoutKv);
+        return false;
+      }
     }
   }
+}
+__device__ __forceinline__ bool kv_wait(uint64_t* bar, uint32_t parity, int* err) {
+  const uint32_t b = smem_u32(bar);
+  return kv_try_wait(b, parity) || kv_wait_on(b, parity, err);
+}
+// The same for a converged warp: met by all its lanes.
+__device__ __forceinline__ bool kv_wait_warp(uint32_t bar, uint32_t parity, int* err) {
+  return __all_sync(0xffffffffu, kv_try_wait(bar, parity)) || __all_sync(0xffffffffu, kv_wait_on(bar, parity, err));
+}
+__device__ __forceinline__ bool kv_wait_warp(uint64_t* bar, uint32_t parity, int* err) {
+  return kv_wait_warp(smem_u32(bar), parity, err);
+}
+
+// Barrier `id` among `threads` threads (whole warps) of the block.
+__device__ __forceinline__ void named_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+// The same, telling whether `v` holds in any of the threads.
+__device__ __forceinline__ bool named_any(int id, int threads, bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %3, 0;\n\t"
+      "barrier.cta.red.or.pred q, %1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"(threads), "r"(static_cast<uint32_t>(v))
+      : "memory");
+  return r != 0;
 }
 
 // Dynamic shared memory limit of a kernel, set once per device.

@@ -17,7 +17,7 @@ namespace dcpp {
 
 // sum_{i < n} floor((a i + b) / m): the Euclid-like floor-sum recurrence (as in
 // the AtCoder Library's floor_sum).  All values below 2^31.
-__device__ __forceinline__ int64_t kv_floor_sum(int64_t n, uint32_t m, uint32_t a, uint32_t b) {
+static __device__ __noinline__ int64_t kv_floor_sum(int64_t n, uint32_t m, uint32_t a, uint32_t b) {
   int64_t ans = 0;
   uint32_t nn = static_cast<uint32_t>(n);
   while (nn > 0) {
@@ -29,10 +29,10 @@ __device__ __forceinline__ int64_t kv_floor_sum(int64_t n, uint32_t m, uint32_t 
       ans += static_cast<int64_t>(nn) * (b / m);
       b %= m;
     }
-    const uint64_t top = static_cast<uint64_t>(a) * nn + b;
+    const uint32_t top = a * nn + b;  // a < m <= 128, nn <= 2^24
     if (top < m) break;
-    nn = static_cast<uint32_t>(top / m);
-    b = static_cast<uint32_t>(top % m);
+    nn = top / m;
+    b = top % m;
     const uint32_t t = m;
     m = a;
     a = t;
@@ -60,7 +60,7 @@ __device__ __forceinline__ KvSeq kv_seq(const KvAttnArgs& p, int b) {
     s.q0 = s.q_len = s.kv = 0;
   }
   s.off = s.kv - s.q_len;
-  s.units = (s.q_len + p.unit_tokens - 1) / p.unit_tokens;
+  s.units = p.unit_shift >= 0 ? (s.q_len + p.unit_tokens - 1) >> p.unit_shift : (s.q_len + p.unit_tokens - 1) / p.unit_tokens;
   return s;
 }
 
@@ -86,11 +86,25 @@ __device__ __forceinline__ int64_t kv_units_before(const KvAttnArgs& p, const Kv
   }
   // Units whose last key lies in the first tile (or before it) count 1.
   const int U = p.unit_tokens;
-  const int ones = s.off + U > KT ? 0 : min(n, (KT - s.off) / U);
+  int ones = 0;
+  if (s.off + U <= KT) ones = min(n, p.unit_shift >= 0 ? (KT - s.off) >> p.unit_shift : (KT - s.off) / U);
   sum += ones;
-  if (n > ones)
-    sum += kv_floor_sum(n - ones, KT, static_cast<uint32_t>(U),
-                        static_cast<uint32_t>(s.off + (ones + 1) * U + KT - 1));
+  if (n > ones) {
+    const int64_t k = n - ones;
+    const uint32_t b = static_cast<uint32_t>(s.off + (ones + 1) * U + KT - 1);
+    if (p.unit_shift < 0) {
+      sum += kv_floor_sum(k, KT, static_cast<uint32_t>(U), b);
+    } else if (U >= KT) {  // powers of two, whole tiles per unit: an arithmetic progression
+      sum += k * (b / KT) + k * (k - 1) / 2 * (U / KT);
+    } else {               // 2^r units per tile: floor((b + i U) / KT) = floor((b / U + i) / 2^r)
+      constexpr int kLog = KT == 64 ? 6 : 7;
+      static_assert(1 << kLog == KT, "tile size");
+      const int r = kLog - p.unit_shift;
+      auto below = [r](int64_t x) { const int64_t q = x >> r; return ((q * (q - 1) / 2) << r) + q * (x - (q << r)); };
+      const int64_t c = b >> p.unit_shift;
+      sum += below(c + k) - below(c);
+    }
+  }
   return sum;
 }
 
@@ -100,9 +114,12 @@ struct KvPos {
   int32_t tile, n_tiles;  // current tile of the unit, tiles of the unit
 };
 
+// The line of tiles and its parts: the first `more` have each + 1 tiles.
 struct KvRange {
   int64_t total;  // tiles in all
+  int64_t each;
   int32_t parts;  // CTAs that have work
+  int32_t more;
 };
 
 // Shared memory of the schedule: per-thread tile sums and the position found.
@@ -113,8 +130,12 @@ struct KvSchedSmem {
   int32_t b;
 };
 
-// First tile of part i of r.parts.
-__device__ __forceinline__ int64_t kv_cut(const KvRange& r, int i) { return r.total * i / r.parts; }
+// First tile of part i of r.parts, and the part that tile `pos` lies in.
+__device__ __forceinline__ int64_t kv_cut(const KvRange& r, int i) { return r.each * i + min(i, r.more); }
+__device__ __forceinline__ int kv_part_of(const KvRange& r, int64_t pos) {
+  const int64_t big = (r.each + 1) * r.more;
+  return static_cast<int>(pos < big ? pos / (r.each + 1) : r.more + (pos - big) / r.each);
+}
 
 // All NT threads of the block: the total, and the position of the tile at
 // pos_of(range) on the line (pos_of may return a value outside [0, total): no
@@ -145,6 +166,14 @@ __device__ __forceinline__ bool kv_locate(const KvAttnArgs& p, KvSchedSmem<NT>& 
   }
   r.total = total;
   r.parts = static_cast<int>(max(static_cast<int64_t>(1), min(static_cast<int64_t>(p.grid), total / MIN_TILES)));
+  if (total >> 32) {
+    r.each = total / r.parts;
+    r.more = static_cast<int>(total - r.each * r.parts);
+  } else {  // the usual case, without a 64-bit division
+    const uint32_t n = static_cast<uint32_t>(total), d = static_cast<uint32_t>(r.parts), q = n / d;
+    r.each = q;
+    r.more = static_cast<int>(n - q * d);
+  }
   const int64_t pos = pos_of(r);
   if (pos < 0 || pos >= total) return false;
   int64_t base = before + incl - mine;
@@ -165,7 +194,8 @@ __device__ __forceinline__ bool kv_locate(const KvAttnArgs& p, KvSchedSmem<NT>& 
   at.s = kv_seq(p, at.b);
   const int64_t per_head = kv_units_before<KT>(p, at.s, at.s.units);
   int64_t rem = pos - sm.base;
-  at.h = static_cast<int>(rem / per_head);
+  at.h = static_cast<int>(rem >> 31 || per_head >> 31 ? rem / per_head
+                                                      : static_cast<int64_t>(static_cast<uint32_t>(rem) / static_cast<uint32_t>(per_head)));
   rem -= at.h * per_head;
   int lo = 0, hi = at.s.units;  // units_before(lo) <= rem < units_before(hi)
   while (hi - lo > 1) {

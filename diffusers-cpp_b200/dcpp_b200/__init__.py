@@ -287,30 +287,34 @@ def _ptr(x) -> Optional[int]:
     raise TypeError(f"cannot take the address of {type(x)}")
 
 
-def _rows(x, device: int, type_: int, cols: int, what: str):
+# torch's dtypes by name, once torch is known to be there (the calls that take tensors need it).
+_DTYPES = {}
+
+
+def _dtypes():
+    if not _DTYPES:
+        import torch
+        _DTYPES.update(i32=torch.int32, i64=torch.int64, f32=torch.float32)
+        _DTYPES[TYPE_F16], _DTYPES[TYPE_BF16] = torch.float16, torch.bfloat16
+    return _DTYPES
+
+
+def _rows(x, device: int, dtype, cols: int, what: str):
     """(address, rows, row stride) of a 2-D or 3-D torch tensor of 16-bit rows on
     `device` whose trailing dimensions are packed and hold `cols` values."""
-    if x.get_device() != device or x.dtype != _torch_dtype(type_):
-        raise DcppError(DCPP_ERR_INVALID_ARG, f"{what}: must be a {_torch_dtype(type_)} tensor on cuda:{device}")
     shape, stride = x.shape, x.stride()
-    packed = (len(shape) == 2 and stride[1] == 1 or
-              len(shape) == 3 and stride[2] == 1 and (stride[1] == shape[2] or shape[1] == 1))
-    if not packed or x.numel() != shape[0] * cols:
-        raise DcppError(DCPP_ERR_INVALID_ARG, f"{what}: must be rows of {cols} packed values")
+    packed = (len(shape) == 2 and stride[1] == 1 and shape[1] == cols or
+              len(shape) == 3 and stride[2] == 1 and (stride[1] == shape[2] or shape[1] == 1) and shape[1] * shape[2] == cols)
+    if x.dtype != dtype or x.get_device() != device or not packed:
+        raise DcppError(DCPP_ERR_INVALID_ARG, f"{what}: must be {dtype} rows of {cols} packed values on cuda:{device}")
     return x.data_ptr(), shape[0], stride[0] if shape[0] > 1 else max(stride[0], cols)
 
 
-def _vec(x, device: int, dtype: str, n: Optional[int], what: str):
-    """Address of a packed torch tensor of `n` values (None: any number) on `device`."""
-    if x.get_device() != device or str(x.dtype) != dtype or not x.is_contiguous() or (n is not None and x.numel() != n):
-        raise DcppError(DCPP_ERR_INVALID_ARG, f"{what}: must be a packed {dtype} tensor on cuda:{device}"
-                        + ("" if n is None else f" of {n} values"))
+def _vec(x, device: int, dtype, n: int, what: str):
+    """Address of a packed torch tensor of `n` values on `device`."""
+    if x.dtype != dtype or x.numel() != n or x.get_device() != device or not x.is_contiguous():
+        raise DcppError(DCPP_ERR_INVALID_ARG, f"{what}: must be a packed {dtype} tensor of {n} values on cuda:{device}")
     return x.data_ptr()
-
-
-def _torch_dtype(type_: int):
-    import torch
-    return torch.float16 if type_ == TYPE_F16 else torch.bfloat16
 
 
 class KVCache:
@@ -333,13 +337,24 @@ class KVCache:
             c.type = TYPE_F16 if k.dtype == torch.float16 else TYPE_BF16
             c.block_size, c.n_blocks, c.heads_kv, c.head_dim, c.block_stride = bs, nb, h, d, max(k.stride(0), h * bs * d)
             c.d_k, c.d_v = k.data_ptr(), v.data_ptr()
-            self.device = k.get_device()
+            self.device, self.dtype = k.get_device(), k.dtype
         else:
             c.block_size, c.n_blocks = block_size, n_blocks
-            self.device = None
+            self.device = self.dtype = None
+        self.n_blocks, self.heads_kv = c.n_blocks, c.heads_kv
         self.k, self.v = k, v  # keeps the storage alive
         self.c = c
         self.ref = ctypes.addressof(c)
+
+
+def _current_stream_handle(device: int) -> int:
+    """Handle of torch's current stream on `device` (0: the default stream), without
+    the cost of a Stream object where torch offers that."""
+    import torch
+    try:
+        return torch._C._cuda_getCurrentRawStream(device)
+    except AttributeError:
+        return torch.cuda.current_stream(device).cuda_stream
 
 
 class Context:
@@ -358,7 +373,8 @@ class Context:
         # (_call): tensors torch has just produced (a .cuda() copy, a fill) are
         # complete before the library reads them, and torch work queued after
         # the call sees its results.
-        self._stream = self._own_stream = None
+        self._own_stream = None
+        self._set_torch_stream(None)
         try:
             import torch
         except ImportError:
@@ -366,7 +382,7 @@ class Context:
         if torch is not None and torch.cuda.is_available():
             self._own_stream = torch.cuda.Stream(device=device)
             self.check(lib().dcpp_set_stream(h, self._own_stream.cuda_stream), "set_stream")
-            self._stream = self._own_stream
+            self._set_torch_stream(self._own_stream)
 
     def check(self, status: int, what: str = ""):
         if status != DCPP_OK:
@@ -395,11 +411,11 @@ class Context:
             self.check(lib().dcpp_set_stream(self.h, stream_ptr), "set_stream")
             if self._own_stream is not None:
                 import torch
-                self._stream = torch.cuda.ExternalStream(stream_ptr, device=self.device)
+                self._set_torch_stream(torch.cuda.ExternalStream(stream_ptr, device=self.device))
         else:
             own = self._own_stream.cuda_stream if self._own_stream is not None else None
             self.check(lib().dcpp_set_stream(self.h, own), "set_stream")
-            self._stream = self._own_stream
+            self._set_torch_stream(self._own_stream)
 
     def use_current_stream(self):
         """Run on torch's current stream, the default stream included: calls made
@@ -408,22 +424,23 @@ class Context:
         s = torch.cuda.current_stream(self.device)
         # The default stream's handle is 0, which the library reads as "its own": name it cudaStreamLegacy.
         self.check(lib().dcpp_set_stream(self.h, s.cuda_stream or 1), "set_stream")
+        self._set_torch_stream(s)
+
+    def _set_torch_stream(self, s):
         self._stream = s
+        self._stream_handle = s.cuda_stream if s is not None else None
 
     def _call(self, fn, *args):
         """fn(*args) (a C entry point that reads or writes device memory),
         ordered with torch's current stream on both sides."""
         s = self._stream
-        if s is None:
+        if s is None or _current_stream_handle(self.device) == self._stream_handle:
             return fn(*args)
         import torch
         cur = torch.cuda.current_stream(self.device)
-        same = cur.cuda_stream == s.cuda_stream
-        if not same:
-            s.wait_stream(cur)
+        s.wait_stream(cur)
         st = fn(*args)
-        if not same:
-            cur.wait_stream(s)
+        cur.wait_stream(s)
         return st
 
     GEMM_AUTO, GEMM_SINGLE_SM, GEMM_PAIR = 0, 1, 2
@@ -487,72 +504,78 @@ class Context:
     # paged key / value cache (torch tensors on the context's GPU)
     ROPE = {"none": 0, "normal": 1, "neox": 2}
 
-    def _on_device(self, cache: "KVCache", what: str):
+    def _dtype_on_device(self, cache: "KVCache", what: str):
         if cache.device != self.device:
             raise DcppError(DCPP_ERR_INVALID_ARG, f"{what}: the cache is not on cuda:{self.device}")
+        return cache.dtype
 
     def kv_plan(self, cache: "KVCache", cached, new, free_blocks, free_in, free_out, block_table, seq_lens, cu_new, slots,
                 positions):
         """Plan one step of cached.numel() requests (dcpp_kv_plan): block_table
         [batch, max_blocks], slots / positions [max_tokens]."""
-        d, batch, rows = self.device, cached.numel(), slots.numel()
-        i32, i64 = "torch.int32", "torch.int64"
+        d, batch, rows, T = self.device, cached.numel(), slots.numel(), _dtypes()
+        i32, i64 = T["i32"], T["i64"]
         if block_table.dim() != 2 or block_table.shape[0] != batch:
             raise DcppError(DCPP_ERR_INVALID_ARG, "kv_plan: block_table must be [batch, max_blocks]")
-        self.check(self._call(
-            lib().dcpp_kv_plan, self.h, cache.ref, batch, _vec(cached, d, i32, batch, "cached"),
-            _vec(new, d, i32, batch, "new"), _vec(free_blocks, d, i32, cache.c.n_blocks, "free_blocks"),
+        width = block_table.shape[1]
+        st = self._call(
+            _LIB.dcpp_kv_plan, self.h, cache.ref, batch, _vec(cached, d, i32, batch, "cached"),
+            _vec(new, d, i32, batch, "new"), _vec(free_blocks, d, i32, cache.n_blocks, "free_blocks"),
             _vec(free_in, d, i64, 2, "free_in"), _vec(free_out, d, i64, 2, "free_out"),
-            _vec(block_table, d, i32, None, "block_table"), block_table.shape[1], _vec(seq_lens, d, i32, batch, "seq_lens"),
+            _vec(block_table, d, i32, batch * width, "block_table"), width, _vec(seq_lens, d, i32, batch, "seq_lens"),
             _vec(cu_new, d, i32, batch + 1, "cu_new"), rows, _vec(slots, d, i32, rows, "slots"),
-            _vec(positions, d, i32, rows, "positions")), "kv_plan")
+            _vec(positions, d, i32, rows, "positions"))
+        if st:
+            self.check(st, "kv_plan")
 
     def kv_store(self, cache: "KVCache", qkv, heads: int, positions, slots, q, norm_q=None, norm_k=None, eps: float = 1e-6,
                  rope: str = "neox", theta: float = 1e6):
         """RMSNorm + rotary embedding of q and k, k and v into the cache (dcpp_kv_store).
         qkv [tokens, (heads + 2 heads_kv) * 128] and q [tokens, heads(, )* 128] may be row-strided."""
-        d, c = self.device, cache.c
-        self._on_device(cache, "kv_store")
-        src, rows, ld = _rows(qkv, d, c.type, (heads + 2 * c.heads_kv) * 128, "qkv")
-        dst, rows_q, ld_q = _rows(q, d, c.type, heads * 128, "q")
+        d, T = self.device, _dtypes()
+        dtype, f32, i32 = self._dtype_on_device(cache, "kv_store"), T["f32"], T["i32"]
+        src, rows, ld = _rows(qkv, d, dtype, (heads + 2 * cache.heads_kv) * 128, "qkv")
+        dst, rows_q, ld_q = _rows(q, d, dtype, heads * 128, "q")
         if rows_q != rows or rope not in self.ROPE:
             raise DcppError(DCPP_ERR_INVALID_ARG, "kv_store: q must have qkv's rows; rope is 'none', 'normal' or 'neox'")
-        f32, i32 = "torch.float32", "torch.int32"
-        self.check(self._call(
-            lib().dcpp_kv_store, self.h, cache.ref, rows, heads, src, ld,
+        st = self._call(
+            _LIB.dcpp_kv_store, self.h, cache.ref, rows, heads, src, ld,
             None if norm_q is None else _vec(norm_q, d, f32, 128, "norm_q"),
             None if norm_k is None else _vec(norm_k, d, f32, 128, "norm_k"), eps, self.ROPE[rope], theta,
             None if positions is None else _vec(positions, d, i32, rows, "positions"), _vec(slots, d, i32, rows, "slots"),
-            dst, ld_q), "kv_store")
+            dst, ld_q)
+        if st:
+            self.check(st, "kv_store")
 
     def kv_attention_workspace(self, cache: "KVCache", heads: int, max_new: int) -> int:
         """Bytes of the workspace kv_attention needs (dcpp_kv_attention_workspace)."""
         out = ctypes.c_size_t()
-        self.check(lib().dcpp_kv_attention_workspace(self.h, cache.ref, heads, max_new, ctypes.byref(out)),
-                   "kv_attention_workspace")
+        st = lib().dcpp_kv_attention_workspace(self.h, cache.ref, heads, max_new, ctypes.byref(out))
+        if st:
+            self.check(st, "kv_attention_workspace")
         return out.value
 
     def kv_attention(self, cache: "KVCache", q, cu_new, seq_lens, block_table, max_new: int, workspace, out,
                      causal: bool = True, scale: Optional[float] = None):
         """Attention of the new tokens over the cache (dcpp_kv_attention): q, out
         [tokens, heads, 128], rows may be strided; scale None: 1 / sqrt(128)."""
-        d, c = self.device, cache.c
-        self._on_device(cache, "kv_attention")
-        if q.dim() != 3 or q.shape != out.shape:
-            raise DcppError(DCPP_ERR_INVALID_ARG, "kv_attention: q and out must be [tokens, heads, 128]")
-        heads, batch = q.shape[1], seq_lens.numel()
-        src, rows, ld = _rows(q, d, c.type, heads * 128, "q")
-        dst, _, ld_out = _rows(out, d, c.type, heads * 128, "out")
-        if block_table.dim() != 2 or block_table.shape[0] != batch:
-            raise DcppError(DCPP_ERR_INVALID_ARG, "kv_attention: block_table must be [batch, max_blocks]")
+        d, i32 = self.device, _dtypes()["i32"]
+        dtype = self._dtype_on_device(cache, "kv_attention")
+        if q.dim() != 3 or q.shape != out.shape or block_table.dim() != 2:
+            raise DcppError(DCPP_ERR_INVALID_ARG, "kv_attention: q and out must be [tokens, heads, 128], block_table "
+                            "[batch, max_blocks]")
+        heads, (batch, width) = q.shape[1], block_table.shape
+        src, rows, ld = _rows(q, d, dtype, heads * 128, "q")
+        dst, _, ld_out = _rows(out, d, dtype, heads * 128, "out")
         if workspace.get_device() != d or not workspace.is_contiguous():
             raise DcppError(DCPP_ERR_INVALID_ARG, f"kv_attention: the workspace must be packed, on cuda:{d}")
-        i32 = "torch.int32"
-        self.check(self._call(
-            lib().dcpp_kv_attention, self.h, cache.ref, batch, rows, heads, src, ld, _vec(cu_new, d, i32, batch + 1, "cu_new"),
-            _vec(seq_lens, d, i32, batch, "seq_lens"), _vec(block_table, d, i32, None, "block_table"), block_table.shape[1],
-            max_new, 1 if causal else 0, 128.0 ** -0.5 if scale is None else scale, workspace.data_ptr(), workspace.nbytes,
-            dst, ld_out), "kv_attention")
+        st = self._call(
+            _LIB.dcpp_kv_attention, self.h, cache.ref, batch, rows, heads, src, ld,
+            _vec(cu_new, d, i32, batch + 1, "cu_new"), _vec(seq_lens, d, i32, batch, "seq_lens"),
+            _vec(block_table, d, i32, batch * width, "block_table"), width, max_new, 1 if causal else 0,
+            128.0 ** -0.5 if scale is None else scale, workspace.data_ptr(), workspace.nbytes, dst, ld_out)
+        if st:
+            self.check(st, "kv_attention")
 
     # tensor parallelism
     @staticmethod
