@@ -85,13 +85,11 @@ __global__ void __launch_bounds__(kRThreads, 2)
   }
   KvRange range;
   KvPos at;
-  const bool have = kv_locate<kRKT, kRThreads, kRMinTiles>(p, sched, range, at, [&](const KvRange& r) {
-    return static_cast<int>(blockIdx.x) < r.parts ? kv_cut(r, blockIdx.x) : static_cast<int64_t>(-1);
-  });
+  int64_t left = kv_share<kRKT, kRThreads, kRMinTiles, 0>(p, sched, range, at);
   __syncthreads();  // barriers initialised
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (!have) return;
-  int64_t left = kv_cut(range, blockIdx.x + 1) - kv_cut(range, blockIdx.x);
+  if (tid == 0) kv_write_cut(p, range, at, left > 0, blockIdx.x);
+  if (left <= 0) return;
 
   if (warp == 4) {
     // Producer: lane -> (K or V, half, box); the block ids come from the table 32 at
@@ -381,104 +379,136 @@ __global__ void __launch_bounds__(kRThreads, 2)
 }
 
 // ------------------------------------------------------------ joining parts
-// Block c looks at the cut between parts c and c + 1.  If it goes through a unit
-// and is the first cut to do so, the block joins that unit's parts, in the order
-// of the parts: the result does not depend on which CTA finished first.  A warp
-// per row, 32 rows per block (the y blocks of a cut share the unit's rows): what it
-// costs is latency, a chain of two loads per row.
+// A unit in the parts f .. l has its partial sums in slot 2 f + 1 (it starts there)
+// and 2 k, k = f + 1 .. l.  They are summed in the order of the parts, so the result
+// does not depend on which CTA finished first.  What this costs is latency, so the
+// work is spread wide: the blocks of all of a unit's cuts (and their y blocks) share
+// its rows, four to a group whose loads go out together; a group is one warp's, or,
+// for a unit in eight parts or more, a block's whose warps take every eighth part each.
 constexpr int kJThreads = 256;
-constexpr int kJRows = 32;
+constexpr int kJWarps = kJThreads / 32;
+constexpr int kJPer = 4;  // rows of a group
 
-template <int KT, int MIN_TILES, bool F16>
-__global__ void __launch_bounds__(kJThreads) kv_join_kernel(const __grid_constant__ KvAttnArgs p, int R) {
-  __shared__ KvSchedSmem<kJThreads> sched;
-  KvRange range;
-  KvPos at;
+__device__ __forceinline__ void join_fma(float4& s, float w, const float4& a) {
+  if (w != 0.f) {  // a part of weight 0 may not have written its sums
+    s.x = fmaf(w, a.x, s.x); s.y = fmaf(w, a.y, s.y);
+    s.z = fmaf(w, a.z, s.z); s.w = fmaf(w, a.w, s.w);
+  }
+}
+
+template <bool F16>
+__device__ __forceinline__ void join_store(const KvAttnArgs& p, const KvCut& cut, int r, int c4, const float4& a, float by) {
+  const int tok = r / p.group, hh = r - tok * p.group;
+  uint16_t* dst = p.out + static_cast<int64_t>(cut.tok0 + tok) * p.ld_out + (cut.head0 + hh) * 128 + c4;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(kv_pack2<F16>(a.x * by, a.y * by), kv_pack2<F16>(a.z * by, a.w * by));
+}
+
+template <bool F16>
+__global__ void __launch_bounds__(kJThreads, 3) kv_join_kernel(const __grid_constant__ KvAttnArgs p, int R) {
+  __shared__ float4 s_sum[kJWarps][kJPer][32];
+  __shared__ float2 s_ml[kJWarps][kJPer];
   const int c = blockIdx.x + 1;
-  const bool have = kv_locate<KT, kJThreads, MIN_TILES>(p, sched, range, at, [&](const KvRange& r) {
-    return c < r.parts ? kv_cut(r, c) : static_cast<int64_t>(-1);
-  });
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (!have || at.tile == 0) return;
-  const int64_t start = kv_cut(range, c) - at.tile;
-  if (kv_cut(range, c - 1) > start) return;  // an earlier cut went through this unit
-  const int64_t end = start + at.n_tiles;
-  const int last = kv_part_of(range, end - 1);
-  const int t0 = at.s.q0 + at.u * p.unit_tokens;
-  const int rows = min(p.unit_tokens, at.s.q_len - at.u * p.unit_tokens) * p.group;
-  const int lane = threadIdx.x & 31, c4 = lane * 4;
-  // Part k's slot: the unit starts in part c - 1, goes on in c .. last.
-  auto row_of = [&](int k, int r) {
-    return (2 * static_cast<int64_t>(k) + (k == c - 1 ? 1 : 0)) * R + r;
-  };
-  // A warp's four rows go through the loads together: each is one chain (maxima and
-  // sums, then the parts), and it is the length of a chain that this kernel costs.
-  constexpr int kPer = kJRows / (kJThreads / 32);
-  const int r0 = blockIdx.y * kJRows + (threadIdx.x >> 5) * kPer;
-  if (r0 >= rows) return;
-  float M[kPer], L[kPer];
-  float4 a[kPer];
+  const KvCut cut = p.cuts[c];
+  if (cut.rows == 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c4 = lane * 4;
+  const int parts = cut.last - cut.first + 1;
+  // This block among those of the unit's parts - 1 cuts.
+  const int block = (c - cut.first - 1) * gridDim.y + blockIdx.y, blocks = (parts - 1) * gridDim.y;
+  const int groups = (cut.rows + kJPer - 1) / kJPer;
+  const int64_t slot0 = 2 * static_cast<int64_t>(cut.first) * R;
+  auto at = [&](int i, int r) { return slot0 + (i == 0 ? 1 : 2 * i) * static_cast<int64_t>(R) + r; };  // part i of the unit, row r
+  if (parts < kJWarps) {
+    for (int g = block * kJWarps + warp; g < groups; g += blocks * kJWarps) {
+      const int r0 = g * kJPer;
+      // Lane 8 q + i: the maximum and sum of row q in part i; their weights from them.
+      const int mi = lane & 7, mq = lane >> 3;
+      const float2 ml = mi < parts && r0 + mq < cut.rows ? p.part_ml[at(mi, r0 + mq)] : make_float2(-INFINITY, 0.f);
+      float4 s[kJPer], a[2][kJPer];
 #pragma unroll
-  for (int q = 0; q < kPer; ++q) {
-    M[q] = -INFINITY;
-    L[q] = 0.f;
-    a[q] = make_float4(0.f, 0.f, 0.f, 0.f);
-  }
-  for (int k0 = c - 1; k0 <= last; k0 += 32) {  // lane i holds the maximum and sum of part k0 + i
-    const int n = min(32, last - k0 + 1);
-    float2 ml[kPer];
-    float w[kPer];
+      for (int q = 0; q < kJPer; ++q) {
+        s[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+        // In bounds for every row of the unit's slot; the first two parts always exist.
+        a[0][q] = *reinterpret_cast<const float4*>(p.part_o + at(0, min(r0 + q, cut.rows - 1)) * 128 + c4);
+        a[1][q] = *reinterpret_cast<const float4*>(p.part_o + at(1, min(r0 + q, cut.rows - 1)) * 128 + c4);
+      }
+      float M = ml.x;
 #pragma unroll
-    for (int q = 0; q < kPer; ++q)
-      ml[q] = lane < n && r0 + q < rows ? p.part_ml[row_of(k0 + lane, r0 + q)] : make_float2(-INFINITY, 0.f);
+      for (int o = 4; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+      float w = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
+      float L = w * ml.y;
 #pragma unroll
-    for (int q = 0; q < kPer; ++q) {
-      float mx = ml[q].x;
+      for (int o = 4; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+      w = L > 0.f ? w / L : 0.f;
+      for (int i = 0; i < parts; i += 2) {
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      const float Mn = fmaxf(M[q], mx);
-      const float ref = Mn == -INFINITY ? 0.f : Mn;  // no key so far: every weight 0
-      const float keep = ex2(M[q] - ref);
-      w[q] = ex2(ml[q].x - ref);
-      float sum = w[q] * ml[q].y;
+        for (int e = 0; e < 2; ++e)
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      L[q] = L[q] * keep + sum;
-      a[q].x *= keep; a[q].y *= keep; a[q].z *= keep; a[q].w *= keep;
-      M[q] = Mn;
-    }
-    for (int i = 0; i < n; i += 2) {
-      float4 v[2][kPer];
-      float wi[2][kPer];
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-#pragma unroll
-        for (int q = 0; q < kPer; ++q) {
-          wi[e][q] = __shfl_sync(0xffffffffu, w[q], min(i + e, 31));
-          if (i + e >= n) wi[e][q] = 0.f;
-          // A part of weight 0 may not have written its sums.
-          if (wi[e][q] != 0.f) v[e][q] = *reinterpret_cast<const float4*>(p.part_o + row_of(k0 + i + e, r0 + q) * 128 + c4);
-        }
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-#pragma unroll
-        for (int q = 0; q < kPer; ++q)
-          if (wi[e][q] != 0.f) {
-            a[q].x = fmaf(wi[e][q], v[e][q].x, a[q].x); a[q].y = fmaf(wi[e][q], v[e][q].y, a[q].y);
-            a[q].z = fmaf(wi[e][q], v[e][q].z, a[q].z); a[q].w = fmaf(wi[e][q], v[e][q].w, a[q].w);
+          for (int q = 0; q < kJPer; ++q) {
+            if (i > 0 && i + e < parts)
+              a[e][q] = *reinterpret_cast<const float4*>(p.part_o + at(i + e, min(r0 + q, cut.rows - 1)) * 128 + c4);
           }
-    }
-  }
 #pragma unroll
-  for (int q = 0; q < kPer; ++q) {
-    const int r = r0 + q;
-    if (r >= rows) break;
-    const float inv = L[q] > 0.f ? 1.0f / L[q] : 0.f;
-    const int tok = r / p.group, hh = r - tok * p.group;
-    uint16_t* dst = p.out + static_cast<int64_t>(t0 + tok) * p.ld_out +
-                    (static_cast<int64_t>(at.h) * p.group + hh) * 128 + c4;
-    *reinterpret_cast<uint2*>(dst) =
-        make_uint2(kv_pack2<F16>(a[q].x * inv, a[q].y * inv), kv_pack2<F16>(a[q].z * inv, a[q].w * inv));
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int q = 0; q < kJPer; ++q) join_fma(s[q], __shfl_sync(0xffffffffu, w, q * 8 + min(i + e, 7)), a[e][q]);
+      }
+#pragma unroll
+      for (int q = 0; q < kJPer; ++q)
+        if (r0 + q < cut.rows) join_store<F16>(p, cut, r0 + q, c4, s[q], 1.0f);
+    }
+    return;
+  }
+  for (int g = block; g < groups; g += blocks) {
+    const int r0 = g * kJPer;
+    float m[kJPer], l[kJPer];
+    float4 s[kJPer];
+#pragma unroll
+    for (int q = 0; q < kJPer; ++q) {
+      m[q] = -INFINITY;
+      l[q] = 0.f;
+      s[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    for (int i = warp; i < parts; i += kJWarps) {
+      float2 ml[kJPer];
+      float4 a[kJPer];
+#pragma unroll
+      for (int q = 0; q < kJPer; ++q) {
+        const int64_t k = at(i, min(r0 + q, cut.rows - 1));
+        ml[q] = p.part_ml[k];
+        a[q] = *reinterpret_cast<const float4*>(p.part_o + k * 128 + c4);
+      }
+#pragma unroll
+      for (int q = 0; q < kJPer; ++q) {
+        const float M = fmaxf(m[q], ml[q].x);
+        if (M == -INFINITY) continue;
+        const float keep = ex2(m[q] - M), w = ml[q].x == -INFINITY ? 0.f : ex2(ml[q].x - M);
+        l[q] = l[q] * keep + w * ml[q].y;
+        s[q].x *= keep; s[q].y *= keep; s[q].z *= keep; s[q].w *= keep;
+        join_fma(s[q], w, a[q]);
+        m[q] = M;
+      }
+    }
+    __syncthreads();  // the group before has been read
+#pragma unroll
+    for (int q = 0; q < kJPer; ++q) {
+      s_sum[warp][q][lane] = s[q];
+      if (lane == 0) s_ml[warp][q] = make_float2(m[q], l[q]);
+    }
+    __syncthreads();
+    if (warp >= kJPer || r0 + warp >= cut.rows) continue;
+    float M = -INFINITY, L = 0.f;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kJWarps; ++w) M = fmaxf(M, s_ml[w][warp].x);
+#pragma unroll
+    for (int w = 0; w < kJWarps; ++w) {
+      const float2 ml = s_ml[w][warp];
+      const float k = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
+      L += k * ml.y;
+      join_fma(sum, k, s_sum[w][warp][lane]);
+    }
+    join_store<F16>(p, cut, r0 + warp, c4, sum, L > 0.f ? 1.0f / L : 0.f);
   }
 }
 
@@ -497,19 +527,19 @@ cudaError_t launch_rows(const KvCacheView& c, KvAttnArgs a, int grid, cudaStream
   return cudaGetLastError();
 }
 
-template <int KT, int MIN_TILES, bool F16>
+template <bool F16>
 cudaError_t launch_join(const KvAttnArgs& a, int rows, cudaStream_t s) {
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(a.grid - 1, (rows + kJRows - 1) / kJRows);
+  cfg.gridDim = dim3(a.grid - 1, std::max(1, rows / (kJPer * kJWarps * 2)));
   cfg.blockDim = dim3(kJThreads);
   cfg.stream = s;
   cudaLaunchAttribute attr{};
-  // May start while the main kernel runs; waits for its end before it reads the parts.
+  // May start while the main kernel runs; waits for its end before it reads anything of it.
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv_join_kernel<KT, MIN_TILES, F16>, a, rows);
+  return cudaLaunchKernelEx(&cfg, kv_join_kernel<F16>, a, rows);
 }
 
 }  // namespace
@@ -578,8 +608,9 @@ KvAttnPlan kv_attention_plan(int heads, int heads_kv, int64_t max_new, int num_s
     pl.grid = num_sms;
   }
   const size_t part_rows = 2 * static_cast<size_t>(pl.grid) * pl.unit_rows;
-  pl.ml_bytes = part_rows * sizeof(float2);  // a multiple of 16
-  pl.bytes = pl.ml_bytes + part_rows * 128 * sizeof(float);
+  pl.cut_bytes = static_cast<size_t>(pl.grid) * sizeof(KvCut);
+  pl.ml_bytes = part_rows * sizeof(float2);  // all multiples of 16
+  pl.bytes = pl.cut_bytes + pl.ml_bytes + part_rows * 128 * sizeof(float);
   return pl;
 }
 
@@ -590,22 +621,22 @@ cudaError_t launch_kv_attention(const KvCacheView& c, KvAttnArgs a, const KvAttn
   for (int i = 0; i <= 8; ++i)
     if (1 << i == plan.unit_tokens) a.unit_shift = i;
   a.grid = plan.grid;
-  a.part_ml = static_cast<float2*>(workspace);
-  a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan.ml_bytes);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  a.cuts = reinterpret_cast<KvCut*>(ws);
+  a.part_ml = reinterpret_cast<float2*>(ws + plan.cut_bytes);
+  a.part_o = reinterpret_cast<float*>(ws + plan.cut_bytes + plan.ml_bytes);
   cudaError_t e;
   if (plan.unit_rows == kTcRows) {
     e = launch_kv_tc(c, a, s);
     if (e != cudaSuccess) return e;
-    return c.f16 ? launch_join<kTcKT, kTcMinTiles, true>(a, plan.unit_rows, s)
-                 : launch_join<kTcKT, kTcMinTiles, false>(a, plan.unit_rows, s);
+    return c.f16 ? launch_join<true>(a, plan.unit_rows, s) : launch_join<false>(a, plan.unit_rows, s);
   }
   if (plan.unit_rows == 16)
     e = c.f16 ? launch_rows<1, true>(c, a, plan.grid, s) : launch_rows<1, false>(c, a, plan.grid, s);
   else
     e = c.f16 ? launch_rows<2, true>(c, a, plan.grid, s) : launch_rows<2, false>(c, a, plan.grid, s);
   if (e != cudaSuccess) return e;
-  return c.f16 ? launch_join<kRKT, kRMinTiles, true>(a, plan.unit_rows, s)
-               : launch_join<kRKT, kRMinTiles, false>(a, plan.unit_rows, s);
+  return c.f16 ? launch_join<true>(a, plan.unit_rows, s) : launch_join<false>(a, plan.unit_rows, s);
 }
 
 }  // namespace dcpp

@@ -198,15 +198,13 @@ __global__ void __launch_bounds__(kTThreads, 1)
   }
   KvRange range;
   KvPos at;
-  const bool have = kv_locate<kTcKT, kTThreads, kTcMinTiles>(p, sched, range, at, [&](const KvRange& r) {
-    return static_cast<int>(blockIdx.x) < r.parts ? kv_cut(r, blockIdx.x) : static_cast<int64_t>(-1);
-  });
+  int64_t left = kv_share<kTcKT, kTThreads, kTcMinTiles, kTcSnap>(p, sched, range, at);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (threadIdx.x == 0) kv_write_cut(p, range, at, left > 0, blockIdx.x);
   const uint32_t tmem = tmem_slot;
-  int64_t left = have ? kv_cut(range, blockIdx.x + 1) - kv_cut(range, blockIdx.x) : 0;
   const int half_tok = p.unit_tokens / 2;
 
   if (warp == 0) {

@@ -57,6 +57,16 @@ struct KvStoreArgs {
 };
 cudaError_t launch_kv_store(const KvStoreArgs& a, bool f16, cudaStream_t s);
 
+// The unit that the cut before a part goes through (rows = 0: none): its parts and
+// where its rows go.
+struct KvCut {
+  int32_t first, last;  // the parts it lies in
+  int32_t rows;
+  int32_t tok0;         // row of q and out of its first token
+  int32_t head0;        // its first query head
+  int32_t pad[3];
+};
+
 // Attention of a batch's new tokens over the cache.
 struct KvAttnArgs {
   const uint16_t* q;        // [tokens, heads, 128], row stride ld_q
@@ -75,6 +85,7 @@ struct KvAttnArgs {
   int32_t unit_tokens;      // query tokens of one work unit
   int32_t unit_shift;       // log2 of it, -1: not a power of two
   int32_t grid;             // CTAs of the main kernel
+  struct KvCut* cuts;       // [grid] what the cut before each part goes through
   float* part_o;            // [2 * grid][unit rows][128] partial sums
   float2* part_ml;          // [2 * grid][unit rows] their running maximum and sum
   int* err;
@@ -85,7 +96,7 @@ struct KvAttnPlan {
   int unit_rows;    // query rows (token, head of the group) of one work unit
   int unit_tokens;
   int grid;
-  size_t ml_bytes, bytes;
+  size_t cut_bytes, ml_bytes, bytes;
 };
 KvAttnPlan kv_attention_plan(int heads, int heads_kv, int64_t max_new, int num_sms);
 

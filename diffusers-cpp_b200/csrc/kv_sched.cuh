@@ -137,11 +137,77 @@ __device__ __forceinline__ int kv_part_of(const KvRange& r, int64_t pos) {
   return static_cast<int>(pos < big ? pos / (r.each + 1) : r.more + (pos - big) / r.each);
 }
 
-// All NT threads of the block: the total, and the position of the tile at
-// pos_of(range) on the line (pos_of may return a value outside [0, total): no
-// position, false).  MIN_TILES: fewest tiles of a part.
-template <int KT, int NT, int MIN_TILES, class PosOf>
-__device__ __forceinline__ bool kv_locate(const KvAttnArgs& p, KvSchedSmem<NT>& sm, KvRange& r, KvPos& at, PosOf pos_of) {
+// All NT threads of the block: the position of the tile at `pos` (on the line).
+// base, mine: first tile and tiles of the thread's run of sequences [b0, b1).
+template <int KT, int NT>
+__device__ __forceinline__ void kv_find(const KvAttnArgs& p, KvSchedSmem<NT>& sm, int64_t base, int64_t mine, int b0, int b1,
+                                        int64_t pos, KvPos& at) {
+  if (pos >= base && pos < base + mine) {
+    for (int b = b0; b < b1; ++b) {
+      const KvSeq s = kv_seq(p, b);
+      const int64_t n = kv_units_before<KT>(p, s, s.units) * p.heads_kv;
+      if (pos < base + n) {
+        sm.b = b;
+        sm.base = base;
+        break;
+      }
+      base += n;
+    }
+  }
+  __syncthreads();
+  at.b = sm.b;
+  int64_t rem = pos - sm.base;
+  at.s = kv_seq(p, at.b);
+  const int64_t per_head = kv_units_before<KT>(p, at.s, at.s.units);
+  at.h = static_cast<int>(rem >> 31 || per_head >> 31 ? rem / per_head
+                                                      : static_cast<int64_t>(static_cast<uint32_t>(rem) / static_cast<uint32_t>(per_head)));
+  rem -= at.h * per_head;
+  int lo = 0, hi = at.s.units;  // units_before(lo) <= rem < units_before(hi)
+  while (hi - lo > 1) {
+    const int step = (hi - lo + NT - 1) / NT;
+    const int64_t cand = static_cast<int64_t>(lo) + static_cast<int64_t>(threadIdx.x) * step;
+    const bool in = cand < hi && kv_units_before<KT>(p, at.s, static_cast<int>(min(cand, static_cast<int64_t>(hi)))) <= rem;
+    const int k = __syncthreads_count(in);  // thread 0 always counts
+    lo += (k - 1) * step;
+    hi = min(hi, lo + step);
+  }
+  at.u = lo;
+  at.tile = static_cast<int>(rem - kv_units_before<KT>(p, at.s, lo));
+  at.n_tiles = kv_unit_tiles<KT>(p, at.s, lo);
+  __syncthreads();  // sm.b and sm.base have been read
+}
+
+// The next unit on the line (false: there is none).
+template <int KT>
+__device__ __forceinline__ bool kv_next_unit(const KvAttnArgs& p, KvPos& at) {
+  at.tile = 0;
+  if (++at.u >= at.s.units) {
+    at.u = 0;
+    if (++at.h >= p.heads_kv) {
+      at.h = 0;
+      do {
+        if (++at.b >= p.batch) return false;
+        at.s = kv_seq(p, at.b);
+      } while (at.s.units == 0);
+    }
+  }
+  at.n_tiles = kv_unit_tiles<KT>(p, at.s, at.u);
+  return true;
+}
+
+// Where a cut that falls on tile `tile` of a unit of n goes: a unit of at most SNAP
+// tiles stays whole, its cut moves to the nearer end.  Returns the move in tiles.
+template <int SNAP>
+__device__ __forceinline__ int kv_snap(int tile, int n) {
+  if (n > SNAP) return 0;
+  return 2 * tile <= n ? -tile : n - tile;
+}
+
+// All NT threads of the block: what this CTA (part blockIdx.x of at most p.grid) has
+// to do, as the position of its first tile and the number of tiles on the line from
+// there (0: nothing).  MIN_TILES: fewest tiles of a part before cuts move.
+template <int KT, int NT, int MIN_TILES, int SNAP>
+__device__ __forceinline__ int64_t kv_share(const KvAttnArgs& p, KvSchedSmem<NT>& sm, KvRange& r, KvPos& at) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int seg = (p.batch + NT - 1) / NT;
   const int b0 = min(tid * seg, p.batch), b1 = min(b0 + seg, p.batch);
@@ -174,60 +240,36 @@ __device__ __forceinline__ bool kv_locate(const KvAttnArgs& p, KvSchedSmem<NT>& 
     r.each = q;
     r.more = static_cast<int>(n - q * d);
   }
-  const int64_t pos = pos_of(r);
-  if (pos < 0 || pos >= total) return false;
-  int64_t base = before + incl - mine;
-  if (pos >= base && pos < base + mine) {
-    for (int b = b0; b < b1; ++b) {
-      const KvSeq s = kv_seq(p, b);
-      const int64_t n = kv_units_before<KT>(p, s, s.units) * p.heads_kv;
-      if (pos < base + n) {
-        sm.b = b;
-        sm.base = base;
-        break;
-      }
-      base += n;
-    }
+  const int c = blockIdx.x;
+  if (c >= r.parts || total == 0) return 0;
+  const int64_t base = before + incl - mine, from = kv_cut(r, c);
+  int64_t to = kv_cut(r, c + 1);
+  if (SNAP > 0 && c + 1 < r.parts) {
+    kv_find<KT, NT>(p, sm, base, mine, b0, b1, to, at);
+    to += kv_snap<SNAP>(at.tile, at.n_tiles);
   }
-  __syncthreads();
-  at.b = sm.b;
-  at.s = kv_seq(p, at.b);
-  const int64_t per_head = kv_units_before<KT>(p, at.s, at.s.units);
-  int64_t rem = pos - sm.base;
-  at.h = static_cast<int>(rem >> 31 || per_head >> 31 ? rem / per_head
-                                                      : static_cast<int64_t>(static_cast<uint32_t>(rem) / static_cast<uint32_t>(per_head)));
-  rem -= at.h * per_head;
-  int lo = 0, hi = at.s.units;  // units_before(lo) <= rem < units_before(hi)
-  while (hi - lo > 1) {
-    const int step = (hi - lo + NT - 1) / NT;
-    const int64_t cand = static_cast<int64_t>(lo) + static_cast<int64_t>(tid) * step;
-    const bool in = cand < hi && kv_units_before<KT>(p, at.s, static_cast<int>(min(cand, static_cast<int64_t>(hi)))) <= rem;
-    const int k = __syncthreads_count(in);  // thread 0 always counts
-    lo += (k - 1) * step;
-    hi = min(hi, lo + step);
-  }
-  at.u = lo;
-  at.tile = static_cast<int>(rem - kv_units_before<KT>(p, at.s, lo));
-  at.n_tiles = kv_unit_tiles<KT>(p, at.s, lo);
-  return true;
+  kv_find<KT, NT>(p, sm, base, mine, b0, b1, from, at);
+  const int move = kv_snap<SNAP>(at.tile, at.n_tiles);
+  if (to <= from + move) return 0;
+  if (move > 0)
+    kv_next_unit<KT>(p, at);
+  else
+    at.tile += move;
+  return to - (from + move);
 }
 
-// The next unit on the line (false: there is none).
-template <int KT>
-__device__ __forceinline__ bool kv_next_unit(const KvAttnArgs& p, KvPos& at) {
-  at.tile = 0;
-  if (++at.u >= at.s.units) {
-    at.u = 0;
-    if (++at.h >= p.heads_kv) {
-      at.h = 0;
-      do {
-        if (++at.b >= p.batch) return false;
-        at.s = kv_seq(p, at.b);
-      } while (at.s.units == 0);
-    }
+// Records what the cut before part `c` goes through, for the kernel that joins parts.
+__device__ __forceinline__ void kv_write_cut(const KvAttnArgs& p, const KvRange& r, const KvPos& at, bool have, int c) {
+  KvCut cut{};
+  if (have && at.tile > 0) {  // such a cut has not been moved
+    const int64_t start = kv_cut(r, c) - at.tile;
+    cut.first = kv_part_of(r, start);
+    cut.last = kv_part_of(r, start + at.n_tiles - 1);
+    cut.rows = min(p.unit_tokens, at.s.q_len - at.u * p.unit_tokens) * p.group;
+    cut.tok0 = at.s.q0 + at.u * p.unit_tokens;
+    cut.head0 = at.h * p.group;
   }
-  at.n_tiles = kv_unit_tiles<KT>(p, at.s, at.u);
-  return true;
+  p.cuts[c] = cut;
 }
 
 }  // namespace dcpp
