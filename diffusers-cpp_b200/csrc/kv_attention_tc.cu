@@ -198,12 +198,12 @@ __global__ void __launch_bounds__(kTThreads, 1)
   }
   KvRange range;
   KvPos at;
-  int64_t left = kv_share<kTcKT, kTThreads, kTcMinTiles, kTcSnap>(p, sched, range, at);
+  int64_t left = p.direct ? max(kv_direct<kTcKT>(p, 1, 0, at), static_cast<int64_t>(0)) : kv_share<kTcKT, kTThreads, kTcMinTiles>(p, sched, range, at);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (threadIdx.x == 0) kv_write_cut(p, range, at, left > 0, blockIdx.x);
+  if (threadIdx.x == 0 && !p.direct) kv_write_cut(p, range, at, left > 0, blockIdx.x);
   const uint32_t tmem = tmem_slot;
   const int half_tok = p.unit_tokens / 2;
 
@@ -561,7 +561,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
 }
 
 template <bool F16>
-cudaError_t launch_tc_t(const KvCacheView& c, KvAttnArgs a, cudaStream_t s) {
+cudaError_t launch_tc_t(const KvCacheView& c, KvAttnArgs a, int ctas, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
   cudaError_t e = allow_smem(kv_tc_kernel<F16>, kTSmem, done);
   if (e != cudaSuccess) return e;
@@ -571,14 +571,14 @@ cudaError_t launch_tc_t(const KvCacheView& c, KvAttnArgs a, cudaStream_t s) {
   if (e == cudaSuccess) e = kv_cache_map(&mk, c, c.k, a.box_rows);
   if (e == cudaSuccess) e = kv_cache_map(&mv, c, c.v, a.box_rows);
   if (e != cudaSuccess) return e;
-  kv_tc_kernel<F16><<<a.grid, kTThreads, kTSmem, s>>>(mq, mk, mv, a);
+  kv_tc_kernel<F16><<<ctas, kTThreads, kTSmem, s>>>(mq, mk, mv, a);
   return cudaGetLastError();
 }
 
 }  // namespace
 
-cudaError_t launch_kv_tc(const KvCacheView& c, KvAttnArgs a, cudaStream_t s) {
-  return c.f16 ? launch_tc_t<true>(c, a, s) : launch_tc_t<false>(c, a, s);
+cudaError_t launch_kv_tc(const KvCacheView& c, KvAttnArgs a, int ctas, cudaStream_t s) {
+  return c.f16 ? launch_tc_t<true>(c, a, ctas, s) : launch_tc_t<false>(c, a, ctas, s);
 }
 
 }  // namespace dcpp

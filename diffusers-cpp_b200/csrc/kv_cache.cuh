@@ -84,7 +84,8 @@ struct KvAttnArgs {
   float scale_log2;         // scale * log2(e)
   int32_t unit_tokens;      // query tokens of one work unit
   int32_t unit_shift;       // log2 of it, -1: not a power of two
-  int32_t grid;             // CTAs of the main kernel
+  int32_t grid;             // parts that the work is cut into, at most
+  int32_t direct;           // > 0: the direct form, units of the longest possible sequence
   struct KvCut* cuts;       // [grid] what the cut before each part goes through
   float* part_o;            // [2 * grid][unit rows][128] partial sums
   float2* part_ml;          // [2 * grid][unit rows] their running maximum and sum

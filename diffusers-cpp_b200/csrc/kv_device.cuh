@@ -106,7 +106,7 @@ cudaError_t kv_query_map(CUtensorMap* m, const KvAttnArgs& a, bool f16, int box_
 constexpr int kTcKT = 128;         // keys of a tile
 constexpr int kTcRows = 256;       // query rows of a unit: two tiles of 128
 constexpr int kTcMinTiles = 4;     // fewest key tiles of a part
-constexpr int kTcSnap = 8;         // units of at most so many key tiles are not cut: joining parts costs about as much
-cudaError_t launch_kv_tc(const KvCacheView& c, KvAttnArgs a, cudaStream_t s);
+constexpr int kTcDirectTiles = 8;  // longest unit of the direct form
+cudaError_t launch_kv_tc(const KvCacheView& c, KvAttnArgs a, int ctas, cudaStream_t s);
 
 }  // namespace dcpp

@@ -195,18 +195,10 @@ __device__ __forceinline__ bool kv_next_unit(const KvAttnArgs& p, KvPos& at) {
   return true;
 }
 
-// Where a cut that falls on tile `tile` of a unit of n goes: a unit of at most SNAP
-// tiles stays whole, its cut moves to the nearer end.  Returns the move in tiles.
-template <int SNAP>
-__device__ __forceinline__ int kv_snap(int tile, int n) {
-  if (n > SNAP) return 0;
-  return 2 * tile <= n ? -tile : n - tile;
-}
-
 // All NT threads of the block: what this CTA (part blockIdx.x of at most p.grid) has
 // to do, as the position of its first tile and the number of tiles on the line from
-// there (0: nothing).  MIN_TILES: fewest tiles of a part before cuts move.
-template <int KT, int NT, int MIN_TILES, int SNAP>
+// there (0: nothing).  MIN_TILES: fewest tiles of a part.
+template <int KT, int NT, int MIN_TILES>
 __device__ __forceinline__ int64_t kv_share(const KvAttnArgs& p, KvSchedSmem<NT>& sm, KvRange& r, KvPos& at) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int seg = (p.batch + NT - 1) / NT;
@@ -243,25 +235,32 @@ __device__ __forceinline__ int64_t kv_share(const KvAttnArgs& p, KvSchedSmem<NT>
   const int c = blockIdx.x;
   if (c >= r.parts || total == 0) return 0;
   const int64_t base = before + incl - mine, from = kv_cut(r, c);
-  int64_t to = kv_cut(r, c + 1);
-  if (SNAP > 0 && c + 1 < r.parts) {
-    kv_find<KT, NT>(p, sm, base, mine, b0, b1, to, at);
-    to += kv_snap<SNAP>(at.tile, at.n_tiles);
-  }
   kv_find<KT, NT>(p, sm, base, mine, b0, b1, from, at);
-  const int move = kv_snap<SNAP>(at.tile, at.n_tiles);
-  if (to <= from + move) return 0;
-  if (move > 0)
-    kv_next_unit<KT>(p, at);
-  else
-    at.tile += move;
-  return to - (from + move);
+  return kv_cut(r, c + 1) - from;
+}
+
+// The direct form, for short units: each cluster of `cluster` CTAs (or each CTA) has
+// one unit (long ones of all sequences first), each CTA an equal run of its tiles.
+// Nothing has to be summed up or searched.  Returns this CTA's tiles; -1: there is no
+// such unit.
+template <int KT>
+__device__ __forceinline__ int64_t kv_direct(const KvAttnArgs& p, int cluster, int rank, KvPos& at) {
+  const int per_unit = p.batch * p.heads_kv, i = blockIdx.x / cluster;
+  const int u = i / per_unit, rest = i - u * per_unit;
+  at.b = rest / p.heads_kv;
+  at.h = rest - at.b * p.heads_kv;
+  at.u = p.direct - 1 - u;
+  at.s = kv_seq(p, at.b);
+  if (at.u >= at.s.units) return -1;
+  at.n_tiles = kv_unit_tiles<KT>(p, at.s, at.u);
+  at.tile = at.n_tiles * rank / cluster;
+  return at.n_tiles * (rank + 1) / cluster - at.tile;
 }
 
 // Records what the cut before part `c` goes through, for the kernel that joins parts.
 __device__ __forceinline__ void kv_write_cut(const KvAttnArgs& p, const KvRange& r, const KvPos& at, bool have, int c) {
   KvCut cut{};
-  if (have && at.tile > 0) {  // such a cut has not been moved
+  if (have && at.tile > 0) {
     const int64_t start = kv_cut(r, c) - at.tile;
     cut.first = kv_part_of(r, start);
     cut.last = kv_part_of(r, start + at.n_tiles - 1);

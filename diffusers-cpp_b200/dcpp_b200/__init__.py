@@ -302,17 +302,22 @@ def _dtypes():
 def _rows(x, device: int, dtype, cols: int, what: str):
     """(address, rows, row stride) of a 2-D or 3-D torch tensor of 16-bit rows on
     `device` whose trailing dimensions are packed and hold `cols` values."""
-    shape, stride = x.shape, x.stride()
-    packed = (len(shape) == 2 and stride[1] == 1 and shape[1] == cols or
-              len(shape) == 3 and stride[2] == 1 and (stride[1] == shape[2] or shape[1] == 1) and shape[1] * shape[2] == cols)
-    if x.dtype != dtype or x.get_device() != device or not packed:
+    if x.dim() == 3:
+        rows, h, d = x.shape
+        ld, sh, sd = x.stride()
+        packed = sd == 1 and (sh == d or h == 1) and h * d == cols
+    else:
+        rows, d = x.shape
+        ld, sd = x.stride()
+        packed = sd == 1 and d == cols
+    if not packed or x.dtype is not dtype or x.get_device() != device:
         raise DcppError(DCPP_ERR_INVALID_ARG, f"{what}: must be {dtype} rows of {cols} packed values on cuda:{device}")
-    return x.data_ptr(), shape[0], stride[0] if shape[0] > 1 else max(stride[0], cols)
+    return x.data_ptr(), rows, ld if rows > 1 else max(ld, cols)
 
 
 def _vec(x, device: int, dtype, n: int, what: str):
     """Address of a packed torch tensor of `n` values on `device`."""
-    if x.dtype != dtype or x.numel() != n or x.get_device() != device or not x.is_contiguous():
+    if x.dtype is not dtype or x.numel() != n or x.get_device() != device or not x.is_contiguous():
         raise DcppError(DCPP_ERR_INVALID_ARG, f"{what}: must be a packed {dtype} tensor of {n} values on cuda:{device}")
     return x.data_ptr()
 
@@ -342,6 +347,7 @@ class KVCache:
             c.block_size, c.n_blocks = block_size, n_blocks
             self.device = self.dtype = None
         self.n_blocks, self.heads_kv = c.n_blocks, c.heads_kv
+        self.workspaces = {}  # (heads, max_new) -> bytes
         self.k, self.v = k, v  # keeps the storage alive
         self.c = c
         self.ref = ctypes.addressof(c)
@@ -350,11 +356,15 @@ class KVCache:
 def _current_stream_handle(device: int) -> int:
     """Handle of torch's current stream on `device` (0: the default stream), without
     the cost of a Stream object where torch offers that."""
-    import torch
-    try:
-        return torch._C._cuda_getCurrentRawStream(device)
-    except AttributeError:
-        return torch.cuda.current_stream(device).cuda_stream
+    global _raw_stream
+    if _raw_stream is None:
+        import torch
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                              lambda d: torch.cuda.current_stream(d).cuda_stream)
+    return _raw_stream(device)
+
+
+_raw_stream = None
 
 
 class Context:
@@ -549,10 +559,14 @@ class Context:
 
     def kv_attention_workspace(self, cache: "KVCache", heads: int, max_new: int) -> int:
         """Bytes of the workspace kv_attention needs (dcpp_kv_attention_workspace)."""
+        known = cache.workspaces.get((heads, max_new))
+        if known is not None:
+            return known
         out = ctypes.c_size_t()
         st = lib().dcpp_kv_attention_workspace(self.h, cache.ref, heads, max_new, ctypes.byref(out))
         if st:
             self.check(st, "kv_attention_workspace")
+        cache.workspaces[heads, max_new] = out.value
         return out.value
 
     def kv_attention(self, cache: "KVCache", q, cu_new, seq_lens, block_table, max_new: int, workspace, out,
