@@ -158,6 +158,7 @@ dcpp_status dcpp_kv_store(dcpp_ctx* ctx, const dcpp_kv_cache* cache, int64_t tok
     if (!(d_q == d_qkv && ld_q == ld_qkv) && overlap(d_qkv, (tokens - 1) * ld_qkv + cols, d_q, (tokens - 1) * ld_q + heads * dcpp::kKvHeadDim))
       bad(kName, "q must be apart from qkv, or be its own q columns");
     if (!d_slots || (rope != DCPP_ROPE_NONE && !d_positions)) bad(kName, "null pointer");
+    if (!aligned(d_norm_q, 16) || !aligned(d_norm_k, 16)) bad(kName, "norm_q and norm_k must be 16-byte aligned");
     a.qkv = d_qkv;
     a.q = d_q;
     a.k = static_cast<uint16_t*>(cache->d_k);
@@ -180,7 +181,7 @@ dcpp_status dcpp_kv_store(dcpp_ctx* ctx, const dcpp_kv_cache* cache, int64_t tok
       const double base = std::log(static_cast<double>(theta));
       for (int i = 0; i < 64; ++i) a.turns[i] = std::exp(-base * i / 64.0) / (2.0 * M_PI);
     }
-    dcpp::cuda_check(dcpp::launch_kv_store(a, cache->type == DCPP_TYPE_F16, ctx->stream), kName);
+    dcpp::cuda_check(dcpp::launch_kv_store(a, cache->type == DCPP_TYPE_F16, ctx->num_sms, ctx->stream), kName);
   });
 }
 

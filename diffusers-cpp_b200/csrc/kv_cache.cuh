@@ -55,7 +55,7 @@ struct KvStoreArgs {
   int* err;
   double turns[64];        // turns per position of pair i: theta^(-i / 64) / (2 pi)
 };
-cudaError_t launch_kv_store(const KvStoreArgs& a, bool f16, cudaStream_t s);
+cudaError_t launch_kv_store(const KvStoreArgs& a, bool f16, int num_sms, cudaStream_t s);
 
 // The unit that the cut before a part goes through (rows = 0: none): its parts and
 // where its rows go.

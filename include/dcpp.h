@@ -276,8 +276,8 @@ dcpp_status dcpp_kv_plan(dcpp_ctx* ctx, const dcpp_kv_cache* cache, int64_t batc
  * norm_q / norm_k [128] f32, NULL: no normalisation.  Pair i turns by position *
  * theta^(-i / 64), the angle in 64 bits.  Rows with slot < 0 are skipped (q too);
  * a slot outside the cache is skipped and reported by dcpp_synchronize
- * (DCPP_ERR_INVALID_ARG).  Slots must be distinct.  Rows and planes: 16-byte
- * aligned, strides multiples of 8. */
+ * (DCPP_ERR_INVALID_ARG).  Slots must be distinct.  Rows, planes and weights:
+ * 16-byte aligned, strides multiples of 8. */
 dcpp_status dcpp_kv_store(dcpp_ctx* ctx, const dcpp_kv_cache* cache, int64_t tokens, int64_t heads,
                           const uint16_t* d_qkv, int64_t ld_qkv, const float* d_norm_q, const float* d_norm_k,
                           float eps, int rope, float theta, const int32_t* d_positions, const int32_t* d_slots,
