@@ -97,29 +97,28 @@ __device__ __forceinline__ bool tc_wait(uint32_t bar, uint32_t phase, int* err) 
   return kv_wait_warp(bar, phase & 1, err);
 }
 
-// What a CTA does with the unit at `at`: its key tiles [first, last), and the steps
-// of 64 keys, from 2 first on, that each row tile needs of them.
+// What tile x of a CTA does with the unit at `at`, whose key tiles [first, last) are the
+// CTA's: n_tok tokens, and the steps of 64 keys from 2 first up to end.
 struct TcWork {
   int first, last;
-  int end[2];  // in steps of 64 keys
-  int tok0, n_tok[2];  // first token of the unit, tokens of each tile
+  int end;
+  int tok0, n_tok;  // first token of the unit, tokens of the tile
+  bool two;         // the unit has a tile B
 };
 
-__device__ __forceinline__ TcWork tc_work(const KvAttnArgs& p, const KvPos& at, int64_t left) {
+__device__ __forceinline__ TcWork tc_work(const KvAttnArgs& p, const KvPos& at, int64_t left, int x) {
   TcWork w;
   const int half = p.unit_tokens / 2;
   w.first = at.tile;
   w.last = at.tile + static_cast<int>(min(left, static_cast<int64_t>(at.n_tiles - at.tile)));
   w.tok0 = at.u * p.unit_tokens;
   const int n = min(p.unit_tokens, at.s.q_len - w.tok0);
-#pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    w.n_tok[x] = min(max(n - x * half, 0), half);
-    int keys = at.s.kv;
-    if (p.causal) keys = min(keys, at.s.off + w.tok0 + x * half + w.n_tok[x]);
-    const int steps = w.n_tok[x] > 0 ? max(1, (keys + 63) >> 6) : 0;
-    w.end[x] = max(2 * w.first, min(2 * w.last, steps));
-  }
+  w.two = n > half;
+  w.n_tok = min(max(n - x * half, 0), half);
+  int keys = at.s.kv;
+  if (p.causal) keys = min(keys, at.s.off + w.tok0 + x * half + w.n_tok);
+  const int steps = w.n_tok > 0 ? max(1, (keys + 63) >> 6) : 0;
+  w.end = max(2 * w.first, min(2 * w.last, steps));
   return w;
 }
 
@@ -216,13 +215,13 @@ __global__ void __launch_bounds__(kTThreads, 1)
     int issued[2] = {0, 0};        // copies of K and of V
     bool ok = true;
     while (left > 0 && ok) {
-      const TcWork w = tc_work(p, at, left);
+      const TcWork w = tc_work(p, at, left, 0);
       ok = kv_wait_warp(&bar.q_empty, (unit & 1) ^ 1, p.err);
       if (!ok) break;
       if (lane == 0) {
-        mbar_arrive_expect_tx(&bar.q_full, w.n_tok[1] > 0 ? 2 * q_bytes : q_bytes);
+        mbar_arrive_expect_tx(&bar.q_full, w.two ? 2 * q_bytes : q_bytes);
         for (int x = 0; x < 2; ++x)
-          if (w.n_tok[x] > 0)
+          if (x == 0 || w.two)
             for (int k = 0; k < 2; ++k)
               tma_load_3d(sQ + x * kTTile + k * kTHalf, &tmQ, &bar.q_full, k * 64, at.h * p.group,
                           at.s.q0 + w.tok0 + x * half_tok);
@@ -297,9 +296,9 @@ __global__ void __launch_bounds__(kTThreads, 1)
     int tk = 0, tv = 0;            // tiles whose K, and whose V, this warp is done with
     bool ok = true;
     while (left > 0 && ok) {
-      const TcWork w = tc_work(p, at, left);
-      const int s0 = 2 * w.first, end = w.end[x], tiles = w.last - w.first;
-      const bool twice = w.n_tok[1] == 0;  // without a tile B, tile A's warp arrives for both
+      const TcWork w = tc_work(p, at, left, x);
+      const int s0 = 2 * w.first, end = w.end, tiles = w.last - w.first;
+      const bool twice = !w.two;  // without a tile B, tile A's warp arrives for both
       // Both warps meet every phase of the barriers in order, used or not: a parity
       // wait tells a phase only from its neighbours.
       if (!(ok = kv_wait_warp(&bar.q_full, unit & 1, p.err))) break;
@@ -386,9 +385,9 @@ __global__ void __launch_bounds__(kTThreads, 1)
       int first, end, keys, limit, all_below;
       {
         const KvPos u = st.at;
-        const TcWork w = tc_work(p, u, st.left);
+        const TcWork w = tc_work(p, u, st.left, x);
         first = 2 * w.first;
-        end = w.end[x];
+        end = w.end;
         const int tile0 = u.s.off + w.tok0 + x * half_tok;  // position of the tile's first token
         keys = u.s.kv;
         limit = u.s.kv;  // keys this row attends to: [0, limit)
@@ -484,11 +483,12 @@ __global__ void __launch_bounds__(kTThreads, 1)
       }
       if (ok && first < end) ok = kv_wait_warp(pv_done + 8 * ((n - 1) & 1), ((n - 1) >> 1) & 1, p.err);
       if (!ok) break;
+      if (l != l) m = l;  // scores that are NaN do not raise the maximum: the row is NaN, not empty
       const KvPos u = st.at;
-      const TcWork w = tc_work(p, u, st.left);
+      const TcWork w = tc_work(p, u, st.left, x);
       const int tok_in = row / p.group, head_in = row - tok_in * p.group;
       const int tok = w.tok0 + x * half_tok + tok_in;
-      const bool mine = tok_in < w.n_tok[x];
+      const bool mine = tok_in < w.n_tok;
       const bool whole = w.first == 0 && w.last == u.n_tiles;
       // A lane holds a row; a store of one row per lane would touch 32 lines with 16
       // bytes each.  So eight lanes trade 16-byte pieces until each holds the same

@@ -70,18 +70,11 @@ __device__ __forceinline__ void named_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
-// The same, telling whether `v` holds in any of the threads.
-__device__ __forceinline__ bool named_any(int id, int threads, bool v) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.b32 p, %3, 0;\n\t"
-      "barrier.cta.red.or.pred q, %1, %2, p;\n\t"
-      "selp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(r)
-      : "r"(id), "r"(threads), "r"(static_cast<uint32_t>(v))
-      : "memory");
-  return r != 0;
+// The maximum; NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 
 // Dynamic shared memory limit of a kernel, set once per device.

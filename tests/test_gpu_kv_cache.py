@@ -198,6 +198,35 @@ def test_store_matches_reference(ctx, dtype, rope, tokens, heads, heads_kv, bloc
     store_case(ctx, tokens, heads, heads_kv, block, dtype, rope, norm, seed=tokens)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("rope", ["neox", "normal", "none"])
+@pytest.mark.parametrize("heads,heads_kv,norm,in_place", [(28, 4, True, False), (5, 1, False, True), (1, 1, True, True), (40, 8, True, True)])
+def test_store_many_tokens(ctx, dtype, rope, heads, heads_kv, norm, in_place):
+    """Enough tokens that warps walk them by themselves, with rows of whole slices and of
+    odd ends, strides of their own, and skipped tokens."""
+    for tokens in (7104, 7500):
+        store_case(ctx, tokens, heads, heads_kv, 16, dtype, rope, norm, seed=heads, in_place=in_place, row_pad=8 if in_place else 0,
+                   stride_pad=8, skip=range(3, tokens, 97))
+
+
+def test_store_many_tokens_with_bad_slots(ctx):
+    n = 8000
+    k = torch.zeros(500, 2, 16, 128, dtype=BF16, device="cuda")
+    v = torch.zeros_like(k)
+    qkv = torch.ones(n, 6 * 128, dtype=BF16, device="cuda")
+    q = torch.zeros(n, 2 * 128, dtype=BF16, device="cuda")
+    slots = torch.arange(n, dtype=torch.int32, device="cuda")
+    slots[17], slots[4000] = 8000, 2 ** 31 - 1
+    ctx.kv_store(dcpp_b200.KVCache(k, v), qkv, 2, torch.zeros_like(slots), slots, q, rope="none")
+    with pytest.raises(dcpp_b200.DcppError) as e:
+        ctx.synchronize()
+    assert e.value.status == 1
+    rows = k.transpose(1, 2).flatten(0, 1).flatten(1)
+    good = torch.ones(n, dtype=torch.bool, device="cuda")
+    good[[17, 4000]] = False
+    assert (rows[good] == 1).all() and (rows[~good] == 0).all() and (q[good] == 1).all() and (q[~good] == 0).all()
+
+
 def test_store_far_positions(ctx):
     store_case(ctx, 50, 4, 2, 16, F16, "neox", True, far=1 << 30)
 
@@ -339,6 +368,55 @@ def test_attention_is_repeatable(ctx):
             attend(ctx, s)
             assert torch.equal(first, s.out)
         ctx.synchronize()
+
+
+# A table this wide says that requests may be long, whatever their lengths: units are
+# cut into parts and joined.
+WIDE = 9000
+
+
+@pytest.mark.parametrize("heads,heads_kv", [(32, 8), (16, 2), (8, 8), (12, 4), (64, 1)])
+@pytest.mark.parametrize("new,cached", [([1] * 7, [0, 1, 63, 64, 3000, 127, 128]), ([3, 1, 4], [700, 0, 2000]),
+                                        ([40, 1, 16, 0, 33], [1, 2500, 128, 7, 95]), ([260, 5, 130], [100, 640, 1000])])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_attention_cut_units(ctx, heads, heads_kv, new, cached, dtype):
+    run(ctx, Batch(new, cached, heads, heads_kv, 16, dtype, seed=heads, table_pad=WIDE))
+
+
+@pytest.mark.parametrize("keys", [1, 63, 64, 65, 127, 128, 129, 191, 192, 193, 255, 256, 257, 320, 383, 384, 385, 512, 513, 1000])
+@pytest.mark.parametrize("table_pad", [2, WIDE])
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_one_row_tile(ctx, keys, table_pad, causal):
+    """Units of up to 128 rows, around every length at which the work of their two sides changes."""
+    new = min(keys, 20)
+    run(ctx, Batch([new, 1, new], [keys - new, 3, keys - new + 1], 12, 2, 16, BF16, seed=keys, table_pad=table_pad), causal)
+
+
+@pytest.mark.parametrize("batch,heads,heads_kv", [(150, 4, 4), (700, 2, 1), (40, 16, 2)])
+@pytest.mark.parametrize("table_pad", [2, WIDE])
+def test_attention_many_short_requests(ctx, batch, heads, heads_kv, table_pad):
+    """More units than CTAs, more requests than threads: sides and slots change hands
+    from unit to unit, and units of one and of two row tiles follow one another."""
+    g = torch.Generator().manual_seed(batch)
+    cached = torch.randint(0, 400, (batch,), generator=g).tolist()
+    for hi in (1, 90):
+        new = torch.randint(0, hi + 1, (batch,), generator=g).tolist()
+        run(ctx, Batch(new, cached, heads, heads_kv, 16, BF16, seed=hi, table_pad=table_pad if batch < 700 else min(table_pad, 300)))
+
+
+@pytest.mark.parametrize("new,cached", [([1], [100]), ([1] * 300, [900] * 300), ([1, 1], [9000, 20]), ([20], [400]), ([20], [9000]), ([200], [100])])
+@pytest.mark.parametrize("table_pad", [2, WIDE])
+def test_attention_nan_stays_in_its_row(ctx, new, cached, table_pad):
+    """A query row with a NaN gives a row of NaN, not one of zeros, and no other row changes."""
+    s = Batch(new, cached, 8, 2, 16, BF16, table_pad=table_pad if len(new) < 300 else 2)
+    attend(ctx, s)
+    want = s.out.clone()
+    s.q[s.tokens // 2, 3, 77] = float("nan")
+    want[s.tokens // 2, 3] = float("nan")
+    attend(ctx, s)
+    ctx.synchronize()
+    assert torch.equal(s.out.isnan(), want.isnan())
+    assert torch.equal(s.out.nan_to_num(0.0), want.nan_to_num(0.0))
 
 
 def test_attention_reports_bad_lengths_and_blocks(ctx):
