@@ -17,7 +17,7 @@ namespace dcpp {
 
 // sum_{i < n} floor((a i + b) / m): the Euclid-like floor-sum recurrence (as in
 // the AtCoder Library's floor_sum).  All values below 2^31.
-static __device__ __noinline__ int64_t kv_floor_sum(int64_t n, uint32_t m, uint32_t a, uint32_t b) {
+static __host__ __device__ __noinline__ int64_t kv_floor_sum(int64_t n, uint32_t m, uint32_t a, uint32_t b) {
   int64_t ans = 0;
   uint32_t nn = static_cast<uint32_t>(n);
   while (nn > 0) {
@@ -66,7 +66,7 @@ __device__ __forceinline__ KvSeq kv_seq(const KvAttnArgs& p, int b) {
 
 // Key tiles of unit u: at least one, so that a unit without keys still writes its zeros.
 template <int KT>
-__device__ __forceinline__ int kv_unit_tiles(const KvAttnArgs& p, const KvSeq& s, int u) {
+__host__ __device__ __forceinline__ int kv_unit_tiles(const KvAttnArgs& p, const KvSeq& s, int u) {
   int keys = s.kv;
   if (p.causal) keys = min(keys, s.off + (u + 1) * p.unit_tokens);
   return max(1, (keys + KT - 1) / KT);
@@ -74,7 +74,7 @@ __device__ __forceinline__ int kv_unit_tiles(const KvAttnArgs& p, const KvSeq& s
 
 // sum_{v < u} n(v).
 template <int KT>
-__device__ __forceinline__ int64_t kv_units_before(const KvAttnArgs& p, const KvSeq& s, int u) {
+__host__ __device__ __forceinline__ int64_t kv_units_before(const KvAttnArgs& p, const KvSeq& s, int u) {
   if (u <= 0) return 0;
   const int full = max(1, (s.kv + KT - 1) / KT);
   if (!p.causal) return static_cast<int64_t>(u) * full;
@@ -131,8 +131,8 @@ struct KvSchedSmem {
 };
 
 // First tile of part i of r.parts, and the part that tile `pos` lies in.
-__device__ __forceinline__ int64_t kv_cut(const KvRange& r, int i) { return r.each * i + min(i, r.more); }
-__device__ __forceinline__ int kv_part_of(const KvRange& r, int64_t pos) {
+__host__ __device__ __forceinline__ int64_t kv_cut(const KvRange& r, int i) { return r.each * i + min(i, r.more); }
+__host__ __device__ __forceinline__ int kv_part_of(const KvRange& r, int64_t pos) {
   const int64_t big = (r.each + 1) * r.more;
   return static_cast<int>(pos < big ? pos / (r.each + 1) : r.more + (pos - big) / r.each);
 }

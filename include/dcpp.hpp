@@ -96,6 +96,39 @@ public:
                           axes_dims.data(), theta, out),
            "flash_attn_ext");
     }
+    /* Paged key / value cache, one step of a batch of requests: block tables and row
+     * offsets from the requests' lengths, the new tokens' keys and values into the
+     * cache, and their attention over it (dcpp_kv_plan, dcpp_kv_store,
+     * dcpp_kv_attention); rows are packed. */
+    void kv_plan(const dcpp_kv_cache& cache, int64_t batch, const int32_t* cached, const int32_t* n_new,
+                 int32_t* free_blocks, const int64_t* free_in, int64_t* free_out, int32_t* block_table,
+                 int64_t max_blocks, int32_t* seq_lens, int32_t* cu_new, int64_t max_tokens, int32_t* slots,
+                 int32_t* positions) {
+        ok(dcpp_kv_plan(ctx_, &cache, batch, cached, n_new, free_blocks, free_in, free_out, block_table, max_blocks,
+                        seq_lens, cu_new, max_tokens, slots, positions),
+           "kv_plan");
+    }
+    void kv_store(const dcpp_kv_cache& cache, int64_t tokens, int64_t heads, const uint16_t* qkv, const float* norm_q,
+                  const float* norm_k, float eps, int rope, float theta, const int32_t* positions,
+                  const int32_t* slots, uint16_t* q) {
+        ok(dcpp_kv_store(ctx_, &cache, tokens, heads, qkv, (heads + 2 * cache.heads_kv) * cache.head_dim, norm_q, norm_k,
+                         eps, rope, theta, positions, slots, q, heads * cache.head_dim),
+           "kv_store");
+    }
+    size_t kv_attention_workspace(const dcpp_kv_cache& cache, int64_t heads, int64_t max_new) const {
+        size_t bytes = 0;
+        ok(dcpp_kv_attention_workspace(ctx_, &cache, heads, max_new, &bytes), "kv_attention_workspace");
+        return bytes;
+    }
+    void kv_attention(const dcpp_kv_cache& cache, int64_t batch, int64_t tokens, int64_t heads, const uint16_t* q,
+                      const int32_t* cu_new, const int32_t* seq_lens, const int32_t* block_table, int64_t max_blocks,
+                      int64_t max_new, bool causal, float scale, void* workspace, size_t workspace_bytes,
+                      uint16_t* out) {
+        ok(dcpp_kv_attention(ctx_, &cache, batch, tokens, heads, q, heads * cache.head_dim, cu_new, seq_lens, block_table,
+                             max_blocks, max_new, causal ? 1 : 0, scale, workspace, workspace_bytes, out,
+                             heads * cache.head_dim),
+           "kv_attention");
+    }
     /* The meta backend's AllReduce at a P -> R bridge (ShardingRuntime.hpp:1082-1091). */
     void all_reduce(void* buf, int64_t count, int dtype) { ok(dcpp_allreduce(ctx_, buf, count, dtype), "all_reduce"); }
     /* Join the tensor-parallel group (one process per GPU); rank 0 makes the id. */
