@@ -63,25 +63,6 @@ constexpr int kRSmem = kRStages * kRStageBytes + kRJoinBytes + 1024;
 constexpr int kRMinTiles = 2;
 constexpr int kRDirectTiles = 12;
 
-__device__ __forceinline__ int cluster_size() {
-  uint32_t n;
-  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n));
-  return static_cast<int>(n);
-}
-__device__ __forceinline__ float2 ld_cluster2(uint32_t addr) {
-  float2 v;
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
-  return v;
-}
-__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(addr)
-               : "memory");
-  return v;
-}
-
 // Joins a unit that the CTAs of a cluster computed together: every warp's sums go to
 // its CTA's shared memory (the stages, all read by now), and each CTA adds up the four
 // warps of all CTAs for its share of the 128 output columns, eight lanes to four
@@ -727,16 +708,26 @@ cudaError_t launch_kv_attention(const KvCacheView& c, KvAttnArgs a, const KvAttn
   const int64_t longest = (a.max_kv + (tc ? kTcKT : kRKT) - 1) / (tc ? kTcKT : kRKT);
   const int64_t units = (a.max_new + plan.unit_tokens - 1) / plan.unit_tokens;
   const int64_t all = units * a.batch * a.heads_kv;
-  // Few units of few rows: a cluster of CTAs for each, as large as still fits the GPU at once.
+  // Few units: a cluster of CTAs for each, as large as still fits the GPU at once (clusters
+  // of 8 one to an SM do not fill every SM).
   int cluster = 1;
-  if (!tc)
-    while (cluster < 8 && 2 * cluster * all <= plan.grid && cluster < longest) cluster *= 2;
-  if (longest <= (tc ? kTcDirectTiles : kRDirectTiles * cluster) && all <= (1 << 20)) a.direct = static_cast<int32_t>(units);
+  const int64_t at_once = tc ? plan.grid - plan.grid / 8 : plan.grid;
+  const bool two = tc && std::min<int64_t>(a.max_new, plan.unit_tokens) * a.group > kTcRows / 2;
+  while (cluster < 8 && 2 * cluster * all <= at_once && (two ? 4 * cluster <= longest : cluster < longest)) cluster *= 2;
+  // How long a CTA's share may be.  tcgen05 kernel, in clusters: not much longer than the
+  // cut form's (one of kTcMinTiles or a balanced one); joining units of two row tiles takes
+  // longer.  Measured, cut / clusters: 1 request x 4 tokens x 8 heads a group over 4000 keys
+  // 20.5 / 13.7 us, over 11000 keys 20.5 / 24.4 us; 16 such requests over 4000 keys 26.7 /
+  // 21.5 us, over 7500 keys 34.9 / 32.0 us; 32 tokens over 8000 keys 22.7 / 25.3 us.
+  int64_t most = tc ? kTcDirectTiles : kRDirectTiles;
+  if (tc && cluster > 1)
+    most = std::min<int64_t>(kTcClusterTiles, std::max<int64_t>(kTcMinTiles, all * longest / plan.grid) + (two ? 2 : 4));
+  if (longest <= most * cluster && all <= (1 << 20)) a.direct = static_cast<int32_t>(units);
   if (!a.direct) cluster = 1;
   const int ctas = a.direct ? static_cast<int>(all) * cluster : plan.grid;
   cudaError_t e;
   if (tc)
-    e = launch_kv_tc(c, a, ctas, s);
+    e = launch_kv_tc(c, a, ctas, cluster, s);
   else
     e = c.f16 ? launch_rows<true>(c, a, ctas, cluster, s) : launch_rows<false>(c, a, ctas, cluster, s);
   if (e != cudaSuccess || a.direct) return e;

@@ -36,6 +36,8 @@ constexpr int kTSlots = 2;                // tiles of K and V in flight
 constexpr int kTHalf = 128 * 128;         // 128 rows x 64 channels: 16 KB
 constexpr int kTTile = 2 * kTHalf;        // 128 x 128: 32 KB
 constexpr int kTSmem = (2 + 2 * kTSlots) * kTTile + 1024;
+constexpr int kTLd = 132;                 // f32 row of sums in shared memory, padded: stores without bank conflicts
+static_assert(kTcRows * kTLd * 4 <= (2 + 2 * kTSlots) * kTTile, "sums of a unit in place of its operands");
 constexpr float kTRescale = 8.0f;         // log2 units a row maximum may grow before O is rescaled
 
 struct TcBars {
@@ -156,7 +158,56 @@ struct TcState {
   int tiles;  // key tiles of the runs before this one
 };
 
+// Joins a unit whose key tiles the CTAs of a cluster shared: every CTA's numerators
+// (rows of kTLd f32) and (maximum, sum) lie in its shared memory, and each CTA adds up
+// every cluster-th row, a warp 8 / cluster rows at a time, so that eight loads are on
+// their way together.  Rows of a unit in order of (token, head): tile B follows tile
+// A's half_rows.
 template <bool F16>
+__device__ __forceinline__ void tc_join_cluster(const KvAttnArgs& p, const KvPos& at, uint32_t sums, uint32_t ml, int cluster,
+                                                int rank) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int half_rows = p.unit_tokens / 2 * p.group, tok0 = at.u * p.unit_tokens;
+  const int rows = min(p.unit_tokens, at.s.q_len - tok0) * p.group;
+  const int per = 8 / cluster, shift = 31 - __clz(cluster);
+  for (int r0 = rank * per + warp * per * cluster; r0 < rows; r0 += kTThreads / 32 * per * cluster) {
+    // Slot q: row r0 + q / cluster in CTA q % cluster.
+    const int q = lane & 7, r = min(r0 + (q >> shift), rows - 1);
+    const int at_row = r < half_rows ? r : 128 + r - half_rows;
+    const float2 v = ld_cluster2(mapa_shared(ml + at_row * 8, q & (cluster - 1)));
+    float M = v.x;
+    for (int o = cluster >> 1; o > 0; o >>= 1) M = max_nan(M, __shfl_xor_sync(0xffffffffu, M, o));
+    float w = v.x == -INFINITY ? 0.f : ex2(v.x - M);
+    float L = w * v.y;
+    for (int o = cluster >> 1; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    w = L != 0.f ? w / L : 0.f;
+    float4 a[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      a[k] = ld_cluster4(mapa_shared(sums + __shfl_sync(0xffffffffu, at_row, k) * (kTLd * 4) + lane * 16, k & (cluster - 1)));
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float wk = __shfl_sync(0xffffffffu, w, k);
+      if (wk != 0.f) {  // a part of weight 0 has not written its sums
+        s.x = fmaf(wk, a[k].x, s.x); s.y = fmaf(wk, a[k].y, s.y);
+        s.z = fmaf(wk, a[k].z, s.z); s.w = fmaf(wk, a[k].w, s.w);
+      }
+      if (((k + 1) & (cluster - 1)) == 0) {
+        const int row = r0 + (k >> shift);
+        if (row < rows) {
+          const int tok = row / p.group, head = row - tok * p.group;
+          uint16_t* dst = p.out + static_cast<int64_t>(at.s.q0 + tok0 + tok) * p.ld_out +
+                          (static_cast<int64_t>(at.h) * p.group + head) * 128 + lane * 4;
+          *reinterpret_cast<uint2*>(dst) = make_uint2(kv_pack2<F16>(s.x, s.y), kv_pack2<F16>(s.z, s.w));
+        }
+        s = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    }
+  }
+}
+
+template <bool F16, bool CLUSTER>
 __global__ void __launch_bounds__(kTThreads, 1)
     kv_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ KvAttnArgs p) {
@@ -168,6 +219,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
   __shared__ uint32_t tmem_slot;
   __shared__ TcState state[8];
   __shared__ KvSchedSmem<kTThreads> sched;
+  __shared__ float2 s_ml[CLUSTER ? kTcRows : 1];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -197,12 +249,17 @@ __global__ void __launch_bounds__(kTThreads, 1)
   }
   KvRange range;
   KvPos at;
-  int64_t left = p.direct ? max(kv_direct<kTcKT>(p, 1, 0, at), static_cast<int64_t>(0)) : kv_share<kTcKT, kTThreads, kTcMinTiles>(p, sched, range, at);
+  // The direct form: one unit for each CTA, or for each cluster, whose CTAs share its key
+  // tiles and join their sums through shared memory.
+  const int cluster = CLUSTER ? cluster_size() : 1, rank = CLUSTER ? static_cast<int>(cluster_ctarank()) : 0;
+  int64_t left = CLUSTER || p.direct ? kv_direct<kTcKT>(p, cluster, rank, at) : kv_share<kTcKT, kTThreads, kTcMinTiles>(p, sched, range, at);
+  const bool no_unit = left < 0;
+  left = max(left, static_cast<int64_t>(0));
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (threadIdx.x == 0 && !p.direct) kv_write_cut(p, range, at, left > 0, blockIdx.x);
+  if (!CLUSTER && threadIdx.x == 0 && !p.direct) kv_write_cut(p, range, at, left > 0, blockIdx.x);
   const uint32_t tmem = tmem_slot;
   const int half_tok = p.unit_tokens / 2;
 
@@ -381,6 +438,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
       st.tiles = 0;
     }
     __syncwarp();
+    if (CLUSTER && st.left == 0) s_ml[x * 128 + row] = make_float2(-INFINITY, 0.f);  // nothing of the unit is this CTA's
     while (ok && st.left > 0) {
       int first, end, keys, limit, all_below;
       {
@@ -482,13 +540,32 @@ __global__ void __launch_bounds__(kTThreads, 1)
         m = m_use;
       }
       if (ok && first < end) ok = kv_wait_warp(pv_done + 8 * ((n - 1) & 1), ((n - 1) >> 1) & 1, p.err);
-      if (!ok) break;
+      if (!CLUSTER && !ok) break;
       if (l != l) m = l;  // scores that are NaN do not raise the maximum: the row is NaN, not empty
       const KvPos u = st.at;
       const TcWork w = tc_work(p, u, st.left, x);
       const int tok_in = row / p.group, head_in = row - tok_in * p.group;
       const int tok = w.tok0 + x * half_tok + tok_in;
       const bool mine = tok_in < w.n_tok;
+      if constexpr (CLUSTER) {
+        if (!ok) m = -INFINITY;  // a wait ran out
+        named_sync(1, 256);      // all products of the CTA are done: their operands' place is free
+        s_ml[x * 128 + row] = make_float2(m, m != -INFINITY ? l : 0.f);
+        tc_fence_after();
+        float4* to = reinterpret_cast<float4*>(smem + (x * 128 + row) * (kTLd * 4));
+#pragma unroll 1
+        for (int g = 0; g < 4; ++g) {
+          uint32_t r[32];
+          tmem_ld32(tO + g * 32, r);
+          tmem_ld_wait();
+          if (mine && m != -INFINITY)
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              to[g * 8 + k] = make_float4(__uint_as_float(r[4 * k]), __uint_as_float(r[4 * k + 1]),
+                                          __uint_as_float(r[4 * k + 2]), __uint_as_float(r[4 * k + 3]));
+        }
+        break;
+      }
       const bool whole = w.first == 0 && w.last == u.n_tiles;
       // A lane holds a row; a store of one row per lane would touch 32 lines with 16
       // bytes each.  So eight lanes trade 16-byte pieces until each holds the same
@@ -554,16 +631,21 @@ __global__ void __launch_bounds__(kTThreads, 1)
 
   tc_fence_before();
   __syncthreads();
+  if constexpr (CLUSTER) {
+    cluster_sync();
+    if (!no_unit) tc_join_cluster<F16>(p, state[0].at, smem_u32(smem), smem_u32(s_ml), cluster, rank);
+    cluster_sync();  // nobody's shared memory goes away while it is read
+  }
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
 }
 
-template <bool F16>
-cudaError_t launch_tc_t(const KvCacheView& c, KvAttnArgs a, int ctas, cudaStream_t s) {
+template <bool F16, bool CLUSTER>
+cudaError_t launch_tc_t(const KvCacheView& c, KvAttnArgs a, int ctas, int cluster, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
-  cudaError_t e = allow_smem(kv_tc_kernel<F16>, kTSmem, done);
+  cudaError_t e = allow_smem(kv_tc_kernel<F16, CLUSTER>, kTSmem, done);
   if (e != cudaSuccess) return e;
   a.box_rows = std::min(c.block_size, kTcKT);
   CUtensorMap mq, mk, mv;
@@ -571,14 +653,29 @@ cudaError_t launch_tc_t(const KvCacheView& c, KvAttnArgs a, int ctas, cudaStream
   if (e == cudaSuccess) e = kv_cache_map(&mk, c, c.k, a.box_rows);
   if (e == cudaSuccess) e = kv_cache_map(&mv, c, c.v, a.box_rows);
   if (e != cudaSuccess) return e;
-  kv_tc_kernel<F16><<<ctas, kTThreads, kTSmem, s>>>(mq, mk, mv, a);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(kTThreads);
+  cfg.dynamicSmemBytes = kTSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = cluster;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = CLUSTER ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kv_tc_kernel<F16, CLUSTER>, mq, mk, mv, a);
+}
+
+template <bool F16>
+cudaError_t launch_tc(const KvCacheView& c, const KvAttnArgs& a, int ctas, int cluster, cudaStream_t s) {
+  return cluster > 1 ? launch_tc_t<F16, true>(c, a, ctas, cluster, s) : launch_tc_t<F16, false>(c, a, ctas, 1, s);
 }
 
 }  // namespace
 
-cudaError_t launch_kv_tc(const KvCacheView& c, KvAttnArgs a, int ctas, cudaStream_t s) {
-  return c.f16 ? launch_tc_t<true>(c, a, ctas, s) : launch_tc_t<false>(c, a, ctas, s);
+cudaError_t launch_kv_tc(const KvCacheView& c, KvAttnArgs a, int ctas, int cluster, cudaStream_t s) {
+  return c.f16 ? launch_tc<true>(c, a, ctas, cluster, s) : launch_tc<false>(c, a, ctas, cluster, s);
 }
 
 }  // namespace dcpp

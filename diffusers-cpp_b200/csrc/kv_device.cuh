@@ -77,6 +77,25 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
+__device__ __forceinline__ int cluster_size() {
+  uint32_t n;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n));
+  return static_cast<int>(n);
+}
+__device__ __forceinline__ float2 ld_cluster2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
 // Dynamic shared memory limit of a kernel, set once per device.
 template <class K>
 cudaError_t allow_smem(K* kernel, int bytes, std::atomic<uint64_t>& done) {
@@ -100,6 +119,7 @@ constexpr int kTcKT = 128;         // keys of a tile
 constexpr int kTcRows = 256;       // query rows of a unit: two tiles of 128
 constexpr int kTcMinTiles = 4;     // fewest key tiles of a part
 constexpr int kTcDirectTiles = 8;  // longest unit of the direct form
-cudaError_t launch_kv_tc(const KvCacheView& c, KvAttnArgs a, int ctas, cudaStream_t s);
+constexpr int kTcClusterTiles = 16;  // longest share of a CTA in a cluster
+cudaError_t launch_kv_tc(const KvCacheView& c, KvAttnArgs a, int ctas, int cluster, cudaStream_t s);
 
 }  // namespace dcpp

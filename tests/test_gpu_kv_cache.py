@@ -392,6 +392,17 @@ def test_attention_one_row_tile(ctx, keys, table_pad, causal):
     run(ctx, Batch([new, 1, new], [keys - new, 3, keys - new + 1], 12, 2, 16, BF16, seed=keys, table_pad=table_pad), causal)
 
 
+@pytest.mark.parametrize("heads,heads_kv", [(8, 1), (16, 2), (32, 8), (12, 4)])
+@pytest.mark.parametrize("new,cached", [([4], [700]), ([4, 0, 6], [900, 30, 3]), ([40], [4000]), ([64, 1], [1000, 0]),
+                                        ([33, 2, 0, 17], [2000, 1, 0, 128]), ([6] * 7, [0, 1, 127, 128, 129, 1500, 300]), ([3, 20], [-2, 800])])
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_few_units(ctx, heads, heads_kv, new, cached, causal):
+    """Units shared by the CTAs of a cluster, of every size: some without a key tile for
+    every CTA, requests without rows, rows without keys."""
+    for block in (16, 256):
+        run(ctx, Batch(new, cached, heads, heads_kv, block, F16 if block == 16 else BF16, seed=heads), causal)
+
+
 @pytest.mark.parametrize("batch,heads,heads_kv", [(150, 4, 4), (700, 2, 1), (40, 16, 2)])
 @pytest.mark.parametrize("table_pad", [2, WIDE])
 def test_attention_many_short_requests(ctx, batch, heads, heads_kv, table_pad):
