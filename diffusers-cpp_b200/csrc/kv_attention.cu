@@ -131,7 +131,7 @@ __device__ __forceinline__ void kv_rows_join_cluster(const KvAttnArgs& p, const 
     }
     if (j == 0 && i0 + (tid >> 3) < units) {
       const float inv = L != 0.f ? 1.0f / L : 0.f;
-      const int tok = r / p.group, hh = r - tok * p.group;
+      const int tok = p.row_token(r), hh = r - tok * p.group;
       uint16_t* dst = p.out + static_cast<int64_t>(t0 + tok) * p.ld_out +
                       (static_cast<int64_t>(at.h) * p.group + hh) * 128 + c4;
       *reinterpret_cast<uint2*>(dst) = make_uint2(kv_pack2<F16>(s.x * inv, s.y * inv), kv_pack2<F16>(s.z * inv, s.w * inv));
@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(kRThreads, 2)
       const int r = i >> 4, ch = i & 15;
       uint4 v = make_uint4(0, 0, 0, 0);
       if (r < rows) {
-        const int tok = r / p.group, hh = r - tok * p.group;
+        const int tok = p.row_token(r), hh = r - tok * p.group;
         v = *reinterpret_cast<const uint4*>(p.q + static_cast<int64_t>(t0 + tok) * p.ld_q +
                                             (static_cast<int64_t>(at.h) * p.group + hh) * 128 + ch * 8);
       }
@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(kRThreads, 2)
     for (int e = 0; e < 2; ++e) {
       const int r = g + e * 8;
       int lim = at.s.kv;
-      if (p.causal) lim = min(lim, at.s.off + at.u * p.unit_tokens + r / p.group + 1);
+      if (p.causal) lim = min(lim, at.s.off + at.u * p.unit_tokens + p.row_token(r) + 1);
       limit[e] = lim;
     }
     if (p.causal) min_limit = min(min_limit, at.s.off + at.u * p.unit_tokens + 1);
@@ -399,44 +399,48 @@ __global__ void __launch_bounds__(kRThreads, 2)
     }
     const bool whole = first == 0 && n == at.n_tiles;
     const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (first == 0 ? 1 : 0);
-    constexpr int DC = 32;                    // output columns of a round
-    float* jf = reinterpret_cast<float*>(join);  // [warp][R][DC]
+    // The sums meet in shared memory, 32 columns a round, or all at once where the unit is
+    // the CTA's only one and the stages are free.  Row r of a warp's sums has its 8-column
+    // groups at places ^ (r & 3), so that the four rows of a half warp's stores lie in
+    // different banks.
+    constexpr int ROUNDS = DIRECT ? 1 : 4, DC = 128 / ROUNDS;
+    float* jf = reinterpret_cast<float*>(DIRECT ? smem : join);  // [warp][R][DC]
+    const int r = tid >> 3, c4 = (tid & 7) * 4;
+    const float M = max_nan(max_nan(s_ml[0][r].x, s_ml[1][r].x), max_nan(s_ml[2][r].x, s_ml[3][r].x));
+    float L = 0.f;
 #pragma unroll
-    for (int rd = 0; rd < 128 / DC; ++rd) {
+    for (int k = 0; k < 4; ++k) L += M == -INFINITY ? 0.f : s_ml[k][r].y * ex2(s_ml[k][r].x - M);
+    const float inv = L != 0.f ? 1.0f / L : 0.f;
+    const int tok = p.row_token(r), hh = r - tok * p.group;
+    uint16_t* dst = p.out + static_cast<int64_t>(t0 + tok) * p.ld_out + (static_cast<int64_t>(at.h) * p.group + hh) * 128 + c4;
+    if (!whole && r < rows && c4 == 0) p.part_ml[slot * R + r] = make_float2(M, L);
+#pragma unroll
+    for (int rd = 0; rd < ROUNDS; ++rd) {
 #pragma unroll
       for (int d = 0; d < DC / 8; ++d)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float2 v = make_float2(o[rd * (DC / 8) + d][2 * e] * w[e],
-                                 o[rd * (DC / 8) + d][2 * e + 1] * w[e]);
-          *reinterpret_cast<float2*>(jf + (warp * R + g + e * 8) * DC + d * 8 + cq) = v;
-        }
+        for (int e = 0; e < 2; ++e)
+          *reinterpret_cast<float2*>(jf + (warp * R + g + e * 8) * DC + ((d ^ (g & 3)) << 3) + cq) =
+              make_float2(o[rd * (DC / 8) + d][2 * e] * w[e], o[rd * (DC / 8) + d][2 * e + 1] * w[e]);
       named_sync(1, 128);
-      const int r = tid / (DC / 4), c4 = (tid % (DC / 4)) * 4;
       if (r < rows) {
-        float4 a = *reinterpret_cast<const float4*>(jf + r * DC + c4);
 #pragma unroll
-        for (int k = 1; k < 4; ++k) {
-          const float4 b = *reinterpret_cast<const float4*>(jf + (k * R + r) * DC + c4);
-          a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
-        }
-        const float M = max_nan(max_nan(s_ml[0][r].x, s_ml[1][r].x), max_nan(s_ml[2][r].x, s_ml[3][r].x));
-        float L = 0.f;
+        for (int cc = 0; cc < DC; cc += 32) {
+          const int at_c = cc + (((c4 >> 3) ^ (r & 3)) << 3) + (c4 & 4);
+          float4 a = *reinterpret_cast<const float4*>(jf + r * DC + at_c);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) L += M == -INFINITY ? 0.f : s_ml[k][r].y * ex2(s_ml[k][r].x - M);
-        if (whole) {
-          const float inv = L != 0.f ? 1.0f / L : 0.f;
-          const int tok = r / p.group, hh = r - tok * p.group;
-          uint16_t* dst = p.out + static_cast<int64_t>(t0 + tok) * p.ld_out +
-                          (static_cast<int64_t>(at.h) * p.group + hh) * 128 + rd * DC + c4;
-          *reinterpret_cast<uint2*>(dst) =
-              make_uint2(kv_pack2<F16>(a.x * inv, a.y * inv), kv_pack2<F16>(a.z * inv, a.w * inv));
-        } else {
-          *reinterpret_cast<float4*>(p.part_o + (slot * R + r) * 128 + rd * DC + c4) = a;
-          if (rd == 0 && c4 == 0) p.part_ml[slot * R + r] = make_float2(M, L);
+          for (int k = 1; k < 4; ++k) {
+            const float4 b = *reinterpret_cast<const float4*>(jf + (k * R + r) * DC + at_c);
+            a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+          }
+          const int col = rd * DC + cc;
+          if (whole)
+            *reinterpret_cast<uint2*>(dst + col) = make_uint2(kv_pack2<F16>(a.x * inv, a.y * inv), kv_pack2<F16>(a.z * inv, a.w * inv));
+          else
+            *reinterpret_cast<float4*>(p.part_o + (slot * R + r) * 128 + col + c4) = a;
         }
       }
-      named_sync(1, 128);
+      if (!DIRECT) named_sync(1, 128);
     }
     left -= n;
     if (DIRECT || left <= 0 || !kv_next_unit<kRKT>(p, at)) break;
@@ -465,7 +469,7 @@ __device__ __forceinline__ void join_fma(float4& s, float w, const float4& a) {
 
 template <bool F16>
 __device__ __forceinline__ void join_store(const KvAttnArgs& p, const KvCut& cut, int r, int c4, const float4& a, float by) {
-  const int tok = r / p.group, hh = r - tok * p.group;
+  const int tok = p.row_token(r), hh = r - tok * p.group;
   uint16_t* dst = p.out + static_cast<int64_t>(cut.tok0 + tok) * p.ld_out + (cut.head0 + hh) * 128 + c4;
   *reinterpret_cast<uint2*>(dst) = make_uint2(kv_pack2<F16>(a.x * by, a.y * by), kv_pack2<F16>(a.z * by, a.w * by));
 }
@@ -709,6 +713,7 @@ KvAttnPlan kv_attention_plan(int heads, int heads_kv, int64_t max_new, int num_s
 cudaError_t launch_kv_attention(const KvCacheView& c, KvAttnArgs a, const KvAttnPlan& plan, void* workspace,
                                 cudaStream_t s) {
   a.unit_tokens = plan.unit_tokens;
+  a.group_inv = (65536 + a.group - 1) / a.group;
   a.unit_shift = -1;
   for (int i = 0; i <= 8; ++i)
     if (1 << i == plan.unit_tokens) a.unit_shift = i;

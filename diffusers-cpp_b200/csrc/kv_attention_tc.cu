@@ -201,7 +201,7 @@ __device__ __forceinline__ void tc_join_cluster(const KvAttnArgs& p, const KvPos
       if (((k + 1) & (cluster - 1)) == 0) {
         const int row = r0 + (k >> shift);
         if (row < rows) {
-          const int tok = row / p.group, head = row - tok * p.group;
+          const int tok = p.row_token(row), head = row - tok * p.group;
           uint16_t* dst = p.out + static_cast<int64_t>(at.s.q0 + tok0 + tok) * p.ld_out +
                           (static_cast<int64_t>(at.h) * p.group + head) * 128 + lane * 4;
           *reinterpret_cast<uint2*>(dst) = make_uint2(kv_pack2<F16>(s.x, s.y), kv_pack2<F16>(s.z, s.w));
@@ -454,7 +454,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
         const int tile0 = u.s.off + w.tok0 + x * half_tok;  // position of the tile's first token
         keys = u.s.kv;
         limit = u.s.kv;  // keys this row attends to: [0, limit)
-        if (p.causal) limit = min(limit, tile0 + row / p.group + 1);
+        if (p.causal) limit = min(limit, tile0 + p.row_token(row) + 1);
         all_below = u.s.kv;  // keys that every row of the tile attends to
         if (p.causal) all_below = min(all_below, tile0 + 1);
       }
@@ -549,7 +549,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
       if (l != l) m = l;  // scores that are NaN do not raise the maximum: the row is NaN, not empty
       const KvPos u = st.at;
       const TcWork w = tc_work(p, u, st.left, x);
-      const int tok_in = row / p.group, head_in = row - tok_in * p.group;
+      const int tok_in = p.row_token(row), head_in = row - tok_in * p.group;
       const int tok = w.tok0 + x * half_tok + tok_in;
       const bool mine = tok_in < w.n_tok;
       if constexpr (CLUSTER) {

@@ -90,6 +90,9 @@ struct KvAttnArgs {
   float* part_o;            // [2 * grid][unit rows][128] partial sums
   float2* part_ml;          // [2 * grid][unit rows] their running maximum and sum
   int* err;
+  uint32_t group_inv;       // ceil(2^16 / group)
+  // row / group of a unit's row: its rounding up adds less than 1 / group below 2^16 / group.
+  __host__ __device__ int row_token(int row) const { return static_cast<int>(static_cast<uint32_t>(row) * group_inv >> 16); }
 };
 
 // Geometry of a launch: which kernel runs and the workspace it needs.

@@ -87,6 +87,12 @@ int main() {
         for (int u = 0; u < s.units; ++u) sum += kv_unit_tiles<128>(p, s, u);
         REQUIRE(kv_units_before<128>(p, s, s.units) == sum, "group %d", group);
     }
+    // Division by the group.
+    for (int group = 1; group <= 128; ++group) {
+        KvAttnArgs p{};
+        p.group_inv = (65536 + group - 1) / group;
+        for (int row = 0; row < 256; ++row) REQUIRE(p.row_token(row) == row / group, "group %d row %d", group, row);
+    }
     // The cuts: every tile in one part, parts of equal size but for one tile, and each
     // tile's part found again.
     for (int k = 0; k < 2000; ++k) {
