@@ -174,14 +174,23 @@ __global__ void __launch_bounds__(kRThreads, 2)
   } else {
     left = kv_share<kRKT, kRThreads, kRMinTiles>(p, sched, range, at);
   }
+  // The producer's block ids come from the table 32 at a time, the next 32 fetched ahead;
+  // those of the first tile are on their way while the CTA sets up.
+  int cur = -1, nxt = -1;
+  auto fetch = [&](int i) { return i < p.max_blocks ? __ldg(p.table + at.b * p.max_blocks + i) : -1; };
+  auto fetch_first = [&] {
+    const int win = (at.tile * kRKT) >> p.block_shift;
+    cur = fetch(win + lane);
+    nxt = fetch(win + 32 + lane);
+  };
+  if (warp == 4 && left > 0) fetch_first();
   __syncthreads();  // barriers initialised
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (!DIRECT && tid == 0) kv_write_cut(p, range, at, left > 0, blockIdx.x);
   if (DIRECT ? left < 0 : left == 0) return;
 
   if (warp == 4) {
-    // Producer: lane -> (K or V, half, box); the block ids come from the table 32 at
-    // a time, the next 32 fetched ahead.
+    // Producer: lane -> (K or V, half, box).
     const int boxes = kRKT / p.box_rows;             // 1, 2 or 4 boxes per tile and half
     const int box = lane & (boxes - 1);
     const int part = lane / boxes;                   // 0, 1: K halves; 2, 3: V halves; more: idle
@@ -190,11 +199,7 @@ __global__ void __launch_bounds__(kRThreads, 2)
     bool ok = true;
     while (left > 0 && ok) {
       const int n = static_cast<int>(min(left, static_cast<int64_t>(at.n_tiles - at.tile)));
-      const int32_t* row = p.table + at.b * p.max_blocks;
-      const int n_ids = (at.s.kv + bs_mask) >> p.block_shift;
-      int win = (at.tile * kRKT) >> p.block_shift;   // first block id held
-      auto fetch = [&](int i) { return i < n_ids ? __ldg(row + i) : -1; };
-      int cur = fetch(win + lane), nxt = fetch(win + 32 + lane);
+      int win = (at.tile * kRKT) >> p.block_shift;  // first block id held
       for (int j = at.tile; j < at.tile + n && ok; ++j, ++it) {
         const int key0 = j * kRKT + box * p.box_rows;
         int idx = key0 >> p.block_shift;
@@ -221,6 +226,7 @@ __global__ void __launch_bounds__(kRThreads, 2)
       }
       left -= n;
       if (DIRECT || left <= 0 || !kv_next_unit<kRKT>(p, at)) break;
+      fetch_first();
     }
     // Every copy has landed before the CTA may end (a consumer that gave up waits for none).
     for (int k = max(0, it - kRStages); k < it; ++k)

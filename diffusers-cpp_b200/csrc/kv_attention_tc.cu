@@ -40,7 +40,9 @@ constexpr int kTThreads = 352;
 constexpr int kTSlots = 2;                // tiles of K and V in flight
 constexpr int kTHalf = 128 * 128;         // 128 rows x 64 channels: 16 KB
 constexpr int kTTile = 2 * kTHalf;        // 128 x 128: 32 KB
+constexpr int kTStage = 32 * 128;         // 128 bytes of a warp's rows
 constexpr int kTSmem = (2 + 2 * kTSlots) * kTTile + 1024;
+constexpr int kTSmemOut = kTSmem + 8 * kTStage;  // with the rows on their way out (in clusters they meet in the operands' place)
 constexpr int kTLd = 132;                 // f32 row of sums in shared memory, padded: stores without bank conflicts
 static_assert(kTcRows * kTLd * 4 <= (2 + 2 * kTSlots) * kTTile, "sums of a unit in place of its operands");
 constexpr float kTRescale = 8.0f;         // log2 units a row maximum may grow before O is rescaled
@@ -138,25 +140,6 @@ __device__ __forceinline__ uint4 tc_pack8(const uint32_t* r, float by) {
                     kv_pack2<F16>(__uint_as_float(r[6]) * by, __uint_as_float(r[7]) * by));
 }
 
-// Among eight lanes: lane i's piece k goes to lane k's place i.
-__device__ __forceinline__ void tc_trade8(uint4 (&v)[8], int lane) {
-#pragma unroll
-  for (int s = 1; s < 8; s <<= 1) {
-    const bool up = lane & s;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      if (k & s) continue;
-      const uint4 give = up ? v[k] : v[k | s];
-      uint4 got;
-      got.x = __shfl_xor_sync(0xffffffffu, give.x, s);
-      got.y = __shfl_xor_sync(0xffffffffu, give.y, s);
-      got.z = __shfl_xor_sync(0xffffffffu, give.z, s);
-      got.w = __shfl_xor_sync(0xffffffffu, give.w, s);
-      if (up) v[k] = got; else v[k | s] = got;
-    }
-  }
-}
-
 struct TcState {
   KvPos at;
   int64_t left;
@@ -180,16 +163,16 @@ __device__ __forceinline__ void tc_join_cluster(const KvAttnArgs& p, const KvPos
     const int q = lane & 7, r = min(r0 + (q >> shift), rows - 1);
     const int at_row = r < half_rows ? r : 128 + r - half_rows;
     const float2 v = ld_cluster2(mapa_shared(ml + at_row * 8, q & (cluster - 1)));
+    float4 a[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      a[k] = ld_cluster4(mapa_shared(sums + __shfl_sync(0xffffffffu, at_row, k) * (kTLd * 4) + lane * 16, k & (cluster - 1)));
     float M = v.x;
     for (int o = cluster >> 1; o > 0; o >>= 1) M = max_nan(M, __shfl_xor_sync(0xffffffffu, M, o));
     float w = v.x == -INFINITY ? 0.f : ex2(v.x - M);
     float L = w * v.y;
     for (int o = cluster >> 1; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
     w = L != 0.f ? w / L : 0.f;
-    float4 a[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      a[k] = ld_cluster4(mapa_shared(sums + __shfl_sync(0xffffffffu, at_row, k) * (kTLd * 4) + lane * 16, k & (cluster - 1)));
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
@@ -260,6 +243,16 @@ __global__ void __launch_bounds__(kTThreads, 1)
   int64_t left = CLUSTER || p.direct ? kv_direct<kTcKT>(p, cluster, rank, at) : kv_share<kTcKT, kTThreads, kTcMinTiles>(p, sched, range, at);
   const bool no_unit = left < 0;
   left = max(left, static_cast<int64_t>(0));
+  // The producer's block ids come from the table 32 at a time, the next 32 fetched ahead;
+  // those of the first tile are on their way while the CTA sets up.
+  int cur = -1, nxt = -1;
+  auto fetch = [&](int i) { return i < p.max_blocks ? __ldg(p.table + at.b * p.max_blocks + i) : -1; };
+  auto fetch_first = [&] {
+    const int win = (at.tile * kTcKT) >> p.block_shift;
+    cur = fetch(win + lane);
+    nxt = fetch(win + 32 + lane);
+  };
+  if (warp == 0 && left > 0) fetch_first();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -290,11 +283,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
       }
       __syncwarp();
       ++unit;
-      const int32_t* row = p.table + at.b * p.max_blocks;
-      const int n_ids = (at.s.kv + bs_mask) >> p.block_shift;
       int win = (w.first * kTcKT) >> p.block_shift;
-      auto fetch = [&](int i) { return i < n_ids ? __ldg(row + i) : -1; };
-      int cur = fetch(win + lane), nxt = fetch(win + 32 + lane);
       for (int j = w.first; j < w.last && ok; ++j) {
         const int key0 = j * kTcKT + box * p.box_rows;
         const int idx = key0 >> p.block_shift;
@@ -323,7 +312,10 @@ __global__ void __launch_bounds__(kTThreads, 1)
         ++it;
       }
       left -= w.last - w.first;
-      if (left > 0 && !kv_next_unit<kTcKT>(p, at)) break;
+      if (left > 0) {
+        if (!kv_next_unit<kTcKT>(p, at)) break;
+        fetch_first();
+      }
     }
     // Nothing may be in flight when the CTA ends: all copies landed, and (unless a
     // wait ran out) every slot handed back, i.e. the last commits have arrived.
@@ -437,6 +429,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
     // The walk's state rests in shared memory while a unit is computed: its registers
     // are needed for the scores.
     TcState& st = state[warp - 2];
+    uint8_t* stage = smem + (2 + 2 * kTSlots) * kTTile + (warp - 2) * kTStage;  // 128 bytes of each row on their way out
     if (lane == 0) {
       st.at = at;
       st.left = left;
@@ -573,8 +566,10 @@ __global__ void __launch_bounds__(kTThreads, 1)
       }
       const bool whole = w.first == 0 && w.last == u.n_tiles;
       // A lane holds a row; a store of one row per lane would touch 32 lines with 16
-      // bytes each.  So eight lanes trade 16-byte pieces until each holds the same
-      // piece of all eight rows, and write 128 bytes of a row together.
+      // bytes each.  So the rows go through shared memory, 128 bytes of each at a time
+      // (16-byte pieces at places ^ (row & 7): no bank conflicts), and eight lanes write
+      // a row's 128 bytes together.  (Eight lanes trading their pieces by shuffles cost
+      // three times the instructions: 2 us of 12 for a unit of four key tiles.)
       uint8_t* dst = nullptr;
       if (mine && whole) {
         dst = reinterpret_cast<uint8_t*>(p.out + static_cast<int64_t>(u.s.q0 + tok) * p.ld_out +
@@ -586,40 +581,42 @@ __global__ void __launch_bounds__(kTThreads, 1)
         p.part_ml[at_row] = make_float2(m, m != -INFINITY ? l : 0.f);
         if (m != -INFINITY) dst = reinterpret_cast<uint8_t*>(p.part_o + at_row * 128);  // a part of weight 0 is never read
       }
-      uint8_t* to[8];
+      uint8_t* to[8];  // rows 4 k + lane / 8, this lane's 16 bytes
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        to[k] = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), (lane & 24) + k));
+      for (int k = 0; k < 8; ++k) {
+        to[k] = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), 4 * k + (lane >> 3)));
+        if (to[k]) to[k] += (lane & 7) * 16;
+      }
       tc_fence_after();
       const float inv = m != -INFINITY ? 1.0f / l : 0.f;
+      uint8_t* mine_at = stage + lane * 128;
 #pragma unroll 1
-      for (int g = 0; g < 4; ++g) {  // 32 columns at a time; two of them make a piece of 128 bytes of output
-        uint4 v[8];
-        int at_byte = g * 128;
-        {
-          uint32_t r[32];
+      for (int g = 0; g < 4; ++g) {  // 32 columns at a time; two of them make 128 bytes of output
+        const int at_byte = whole ? g * 64 : g * 128;
+        __syncwarp();  // the pieces before have been read
+        uint32_t r[32];
+        tmem_ld32(tO + g * 32, r);
+        tmem_ld_wait();
+        if (whole) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) *reinterpret_cast<uint4*>(mine_at + ((k ^ (lane & 7)) << 4)) = tc_pack8<F16>(r + k * 8, inv);
+          ++g;
           tmem_ld32(tO + g * 32, r);
           tmem_ld_wait();
-          if (whole) {
-            uint32_t q[32];
-            tmem_ld32(tO + g * 32 + 32, q);
-            tmem_ld_wait();
-            at_byte = g * 64;
-            ++g;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              v[k] = tc_pack8<F16>(r + k * 8, inv);
-              v[4 + k] = tc_pack8<F16>(q + k * 8, inv);
-            }
-          } else {
+          for (int k = 0; k < 4; ++k) *reinterpret_cast<uint4*>(mine_at + (((k + 4) ^ (lane & 7)) << 4)) = tc_pack8<F16>(r + k * 8, inv);
+        } else {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
-          }
+          for (int k = 0; k < 8; ++k)
+            *reinterpret_cast<uint4*>(mine_at + ((k ^ (lane & 7)) << 4)) = make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
         }
-        tc_trade8(v, lane);
+        __syncwarp();
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (to[k]) *reinterpret_cast<uint4*>(to[k] + at_byte + (lane & 7) * 16) = v[k];
+        for (int k = 0; k < 8; ++k) {
+          const int r8 = 4 * k + (lane >> 3);
+          const uint4 v = *reinterpret_cast<const uint4*>(stage + r8 * 128 + (((lane & 7) ^ (r8 & 7)) << 4));
+          if (to[k]) *reinterpret_cast<uint4*>(to[k] + at_byte) = v;
+        }
       }
       tc_fence_before();
       __syncwarp();
@@ -649,8 +646,9 @@ __global__ void __launch_bounds__(kTThreads, 1)
 
 template <bool F16, bool CLUSTER>
 cudaError_t launch_tc_t(const KvCacheView& c, KvAttnArgs a, int ctas, int cluster, cudaStream_t s) {
+  constexpr int smem = CLUSTER ? kTSmem : kTSmemOut;
   static std::atomic<uint64_t> done{0};
-  cudaError_t e = allow_smem(kv_tc_kernel<F16, CLUSTER>, kTSmem, done);
+  cudaError_t e = allow_smem(kv_tc_kernel<F16, CLUSTER>, smem, done);
   if (e != cudaSuccess) return e;
   a.box_rows = std::min(c.block_size, kTcKT);
   CUtensorMap mq, mk, mv;
@@ -661,7 +659,7 @@ cudaError_t launch_tc_t(const KvCacheView& c, KvAttnArgs a, int ctas, int cluste
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(kTThreads);
-  cfg.dynamicSmemBytes = kTSmem;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
