@@ -3,7 +3,7 @@
 //   o[t, h] = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),  s_j = scale q[t, h] . k_j,
 // j over the request's cached keys (causal: up to the token's own position); a row
 // without a key is 0.  Sums, maxima and the scores are f32; the numerators are
-// rounded once to the cache's type (half a step: 2^-9 of each, as the output's own
+// rounded once to the cache's type (half a step: 2^-8 of each in bf16, as the output's own
 // rounding) because the matrix instructions take their operands in it.
 //
 // Rows of one key / value head: the `group` query heads that share it times the
