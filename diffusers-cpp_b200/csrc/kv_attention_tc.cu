@@ -495,8 +495,8 @@ __global__ void __launch_bounds__(kTThreads, 1)
 #pragma unroll
         for (int k = 0; k < 4; ++k) mp[k] = s[k];
 #pragma unroll
-        for (int k = 4; k < 64; k += 2) mp[(k >> 1) & 3] = max3(mp[(k >> 1) & 3], s[k], s[k + 1]);
-        const float mx = c * fmaxf(max3(mp[0], mp[1], mp[2]), mp[3]);
+        for (int k = 4; k < 64; k += 2) mp[(k >> 1) & 3] = max3_nan(mp[(k >> 1) & 3], s[k], s[k + 1]);
+        const float mx = c * max_nan(max3_nan(mp[0], mp[1], mp[2]), mp[3]);
         const bool grow = mx > m + kTRescale;
         const float m_use = grow ? mx : m;
         // A stale maximum is exact (l uses the same one); without a key so far every numerator is 0.
@@ -534,12 +534,13 @@ __global__ void __launch_bounds__(kTThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive_at(p_full + 8 * b);
         const uint64_t t = add2(add2(sp[0], sp[1]), add2(sp[2], sp[3]));
-        l = l * alpha + f2lo(t) + f2hi(t);
+        // A score that is NaN or +inf makes the row NaN, whichever exponential it met.
+        l = mx < INFINITY ? l * alpha + f2lo(t) + f2hi(t) : NAN;
         m = m_use;
       }
       if (ok && first < end) ok = kv_wait_warp(pv_done + 8 * ((n - 1) & 1), ((n - 1) >> 1) & 1, p.err);
       if (!CLUSTER && !ok) break;
-      if (l != l) m = l;  // scores that are NaN do not raise the maximum: the row is NaN, not empty
+      if (l != l) m = l;  // the row is NaN, not empty
       const KvPos u = st.at;
       const TcWork w = tc_work(p, u, st.left, x);
       const int tok_in = p.row_token(row), head_in = row - tok_in * p.group;

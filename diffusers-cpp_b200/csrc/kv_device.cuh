@@ -96,6 +96,12 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
   return v;
 }
 
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // Dynamic shared memory limit of a kernel, set once per device.
 template <class K>
 cudaError_t allow_smem(K* kernel, int bytes, std::atomic<uint64_t>& done) {

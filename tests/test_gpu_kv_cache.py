@@ -430,6 +430,29 @@ def test_attention_nan_stays_in_its_row(ctx, new, cached, table_pad):
     assert torch.equal(s.out.nan_to_num(0.0), want.nan_to_num(0.0))
 
 
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("new,kv", [(1, 70), (20, 150), (150, 200)])
+@pytest.mark.parametrize("table_pad", [2, 600])
+def test_attention_bad_key_reaches_every_row_that_sees_it(ctx, bad, new, kv, table_pad):
+    """A key of NaN, or a score of +inf, at every place in a tile: the rows that attend to
+    it are NaN (as softmax makes them), rows before it and other heads do not change."""
+    n = 130 if new > 1 else kv
+    s = Batch([new] * n, [kv - new] * n, 8, 2, 16, BF16, seed=kv, table_pad=table_pad)
+    s.q[:s.tokens, :4, 5] = 1.0  # of head 0's group: 1 x inf, whatever the other channels
+    attend(ctx, s)
+    want = s.out.clone()
+    first = kv - n if kv - n > 0 else 0
+    for b in range(n):
+        key = (first + b) % kv
+        s.k[s.table[b, key // 16].long(), 0, key % 16, 5] = bad
+        rows = want[s.cu[b] + max(0, key - (kv - new)):s.cu[b + 1]]
+        rows[:, :4] = float("nan")
+    attend(ctx, s)
+    ctx.synchronize()
+    assert torch.equal(s.out.isnan(), want.isnan())
+    assert torch.equal(s.out.nan_to_num(0.0), want.nan_to_num(0.0))
+
+
 def test_attention_reports_bad_lengths_and_blocks(ctx):
     """A request with a bad block or length is reported; the others are computed."""
     for new in ([1, 1, 1], [200, 130, 1]):
