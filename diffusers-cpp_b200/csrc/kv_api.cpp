@@ -208,7 +208,8 @@ dcpp_status dcpp_kv_attention(dcpp_ctx* ctx, const dcpp_kv_cache* cache, int64_t
     check_attention_shape(*cache, heads, max_new, kName);
     if (batch < 1 || tokens < 0 || max_blocks < 1) bad(kName, "batch and max_blocks must be positive, tokens not negative");
     if (batch > (1 << 20) || tokens > (1 << 24)) unsupported(kName, "at most 2^20 requests and 2^24 tokens");
-    if (max_blocks > (INT32_MAX >> a.block_shift)) unsupported(kName, "max_blocks * block_size must fit 31 bits");
+    // A margin, so that sums of a length and a tile's keys fit 32 bits too.
+    if (max_blocks > ((INT32_MAX - 4096) >> a.block_shift)) unsupported(kName, "max_blocks * block_size must stay below 2^31 - 4096");
     if (causal != 0 && causal != 1) bad(kName, "causal must be 0 or 1");
     if (!(scale > 0.0f && std::isfinite(scale))) bad(kName, "scale must be positive");
     if (tokens == 0) return;

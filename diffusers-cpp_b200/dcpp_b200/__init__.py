@@ -306,10 +306,12 @@ def _rows(x, device: int, dtype, cols: int, what: str):
         rows, h, d = x.shape
         ld, sh, sd = x.stride()
         packed = sd == 1 and (sh == d or h == 1) and h * d == cols
-    else:
+    elif x.dim() == 2:
         rows, d = x.shape
         ld, sd = x.stride()
         packed = sd == 1 and d == cols
+    else:
+        packed = False
     if not packed or x.dtype is not dtype or x.get_device() != device:
         raise DcppError(DCPP_ERR_INVALID_ARG, f"{what}: must be {dtype} rows of {cols} packed values on cuda:{device}")
     return x.data_ptr(), rows, ld if rows > 1 else max(ld, cols)
@@ -337,8 +339,9 @@ class KVCache:
                 raise DcppError(DCPP_ERR_INVALID_ARG, "KVCache: k and v must be bf16 or f16 CUDA tensors [n_blocks, "
                                 "heads_kv, block_size, 128] of one layout")
             nb, h, bs, d = k.shape
-            if k.stride()[1:] != (bs * d, d, 1):
-                raise DcppError(DCPP_ERR_INVALID_ARG, "KVCache: the heads, tokens and channels of a block must be packed")
+            if k.stride()[1:] != (bs * d, d, 1) or (nb > 1 and k.stride(0) < h * bs * d):
+                raise DcppError(DCPP_ERR_INVALID_ARG, "KVCache: the heads, tokens and channels of a block must be packed, "
+                                "its blocks apart")
             c.type = TYPE_F16 if k.dtype == torch.float16 else TYPE_BF16
             c.block_size, c.n_blocks, c.heads_kv, c.head_dim, c.block_stride = bs, nb, h, d, max(k.stride(0), h * bs * d)
             c.d_k, c.d_v = k.data_ptr(), v.data_ptr()

@@ -299,9 +299,10 @@ dcpp_status dcpp_kv_store(dcpp_ctx* ctx, const dcpp_kv_cache* cache, int64_t tok
  * Block table entries beyond a request's tokens, and what its last block holds
  * behind them, are never used.  A NaN in a row of q, or in a key that the row
  * attends to, makes the row NaN; a value that causal order hides still meets the
- * weight 0 (0 x inf is NaN), so a request's cached values have to be finite.  Lengths or block ids out of range leave the
- * request's rows undefined and are reported by dcpp_synchronize
- * (DCPP_ERR_INVALID_ARG).  Up to 128 query heads per key / value head. */
+ * weight 0 (0 x inf is NaN), so a request's cached values have to be finite.
+ * Lengths or block ids out of range leave the request's rows undefined and are
+ * reported by dcpp_synchronize (DCPP_ERR_INVALID_ARG).  Up to 128 query heads per
+ * key / value head, max_blocks * block_size below 2^31 - 4096. */
 dcpp_status dcpp_kv_attention_workspace(dcpp_ctx* ctx, const dcpp_kv_cache* cache, int64_t heads, int64_t max_new,
                                         size_t* out_bytes);
 dcpp_status dcpp_kv_attention(dcpp_ctx* ctx, const dcpp_kv_cache* cache, int64_t batch, int64_t tokens, int64_t heads,

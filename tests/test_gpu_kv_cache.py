@@ -564,6 +564,38 @@ def test_plan_refuses(ctx):
     ctx.synchronize()
 
 
+def test_attention_refuses_tables_of_nearly_2_31_keys(ctx):
+    s = Batch([1], [300], 8, 2, 256, BF16)
+    for width, fits in ((8388590, True), (8388600, False)):
+        table = torch.full((1, width), -1, dtype=torch.int32, device="cuda")
+        table[:, :2] = s.table[:, :2]
+        s.table = table
+        if fits:
+            run(ctx, s)
+            continue
+        with pytest.raises(dcpp_b200.DcppError) as e:
+            attend(ctx, s)
+        assert e.value.status == 2
+
+
+def test_layouts_that_share_memory_are_refused(ctx):
+    """Blocks or rows expanded from one: writing them makes no sense, and reading on by
+    the packed size would leave the storage."""
+    one = torch.zeros(1, 2, 16, 128, dtype=BF16, device="cuda")
+    with pytest.raises(dcpp_b200.DcppError) as e:
+        dcpp_b200.KVCache(one.expand(50, -1, -1, -1), one.clone().expand(50, -1, -1, -1))
+    assert e.value.status == 1
+    k = torch.zeros(3, 2, 16, 128, dtype=BF16, device="cuda")
+    cache = dcpp_b200.KVCache(k, k.clone())
+    row = torch.zeros(1, 8 * 128, dtype=BF16, device="cuda")
+    q = torch.zeros(3, 4 * 128, dtype=BF16, device="cuda")
+    for qkv, dst in ((row.expand(3, -1), q), (row.repeat(3, 1), q[:1].expand(3, -1)), (row.flatten(), q)):
+        with pytest.raises(dcpp_b200.DcppError) as e:
+            ctx.kv_store(cache, qkv, 4, ints([0, 1, 2]), ints([0, 1, 2]), dst)
+        assert e.value.status == 1
+    ctx.synchronize()
+
+
 def test_injected_faults_surface(ctx):
     s = Batch([1], [3], 8, 2, 16, BF16)
     for name, call in (("dcpp_kv_attention", lambda: attend(ctx, s)), ("dcpp_kv_plan", lambda: Plan([0], [1], 16, 4, 2, 1).run(ctx))):
