@@ -178,8 +178,18 @@ dcpp_status dcpp_kv_store(dcpp_ctx* ctx, const dcpp_kv_cache* cache, int64_t tok
     a.eps = eps;
     a.err = ctx->d_err;
     if (rope != DCPP_ROPE_NONE) {
+      // theta^(-i / 64) as a product of the powers for i's bits: six exponentials, not 64.
+      // Modulo whole turns (theta < 1 turns faster than once a position).
       const double base = std::log(static_cast<double>(theta));
-      for (int i = 0; i < 64; ++i) a.turns[i] = std::exp(-base * i / 64.0) / (2.0 * M_PI);
+      double bit[6], f[64];
+      for (int b = 0; b < 6; ++b) bit[b] = std::exp(-base * (1 << b) / 64.0);
+      f[0] = 1.0 / (2.0 * M_PI);
+      for (int i = 0; i < 64; ++i) {
+        const int top = i > 0 ? 31 - __builtin_clz(static_cast<unsigned>(i)) : 0;
+        if (i > 0) f[i] = f[i - (1 << top)] * bit[top];
+        const double part = f[i] - std::floor(f[i]);
+        a.turns[i] = static_cast<uint64_t>(std::ldexp(part, 64));
+      }
     }
     dcpp::cuda_check(dcpp::launch_kv_store(a, cache->type == DCPP_TYPE_F16, ctx->num_sms, ctx->stream), kName);
   });

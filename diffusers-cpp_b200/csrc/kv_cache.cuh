@@ -53,7 +53,7 @@ struct KvStoreArgs {
   int32_t rope;            // 0 none, 1 pairs (2i, 2i + 1), 2 pairs (i, i + 64)
   float eps;
   int* err;
-  double turns[64];        // turns per position of pair i: theta^(-i / 64) / (2 pi)
+  uint64_t turns[64];      // 2^64 x the turns per position of pair i, theta^(-i / 64) / (2 pi)
 };
 cudaError_t launch_kv_store(const KvStoreArgs& a, bool f16, int num_sms, cudaStream_t s);
 

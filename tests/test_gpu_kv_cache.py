@@ -204,7 +204,7 @@ def test_store_matches_reference(ctx, dtype, rope, tokens, heads, heads_kv, bloc
 def test_store_many_tokens(ctx, dtype, rope, heads, heads_kv, norm, in_place):
     """Enough tokens that warps walk them by themselves, with rows of whole slices and of
     odd ends, strides of their own, and skipped tokens."""
-    for tokens in (7104, 7500):
+    for tokens in (1184, 1185, 2500, 7500):
         store_case(ctx, tokens, heads, heads_kv, 16, dtype, rope, norm, seed=heads, in_place=in_place, row_pad=8 if in_place else 0,
                    stride_pad=8, skip=range(3, tokens, 97))
 
