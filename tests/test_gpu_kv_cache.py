@@ -721,6 +721,44 @@ def test_step_captured_and_replayed(max_new):
         own.close()
 
 
+@pytest.mark.parametrize("new,cached", [([1, 1], [9000, 20]), ([200, 3, 90], [100, 4000, 0])])
+def test_cut_units_captured_and_replayed(new, cached):
+    """The cut form (two kernels) in a graph, replayed after the lengths have changed: as
+    a call of its own gives."""
+    own = dcpp_b200.Context(0)
+    stream = torch.cuda.Stream()
+    try:
+        s = Batch(new, cached, 16, 4, 16, BF16, table_pad=WIDE)
+        ws = torch.empty(own.kv_attention_workspace(dcpp_b200.KVCache(s.k, s.v), 16, s.max_new), dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            own.use_current_stream()
+            attend(own, s, workspace=ws)
+            own.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                attend(own, s, workspace=ws)
+            for shorter in (0, 1, 700):
+                lens = [max(k - shorter, n) for k, n in zip(s.kv, new)]
+                s.seq_lens.copy_(torch.tensor(lens, dtype=torch.int32))
+                s.out.fill_(7.0)
+                attend(own, s, workspace=ws)
+                want = s.out.clone()
+                s.out.fill_(7.0)
+                ws.fill_(255)
+                graph.replay()
+                own.synchronize()
+                assert torch.equal(s.out, want)
+                assert not torch.equal(s.out[:s.tokens], torch.full_like(s.out[:s.tokens], 7.0))
+            s.kv = lens
+            s.keys, s.values = ([x[:n] for x, n in zip(v, lens)] for v in (s.keys, s.values))
+            s.check()
+        stream.synchronize()
+        del graph
+    finally:
+        own.close()
+
+
 def test_two_streams_with_their_own_workspaces():
     """Two contexts on two streams, each with its own workspace, at the same time."""
     ctxs = [dcpp_b200.Context(0) for _ in range(2)]
