@@ -352,20 +352,21 @@ __global__ void __launch_bounds__(kTThreads, 1)
     while (left > 0 && ok) {
       const TcWork w = tc_work(p, at, left, x);
       const int s0 = 2 * w.first, end = w.end, tiles = w.last - w.first;
-      const bool twice = !w.two;  // without a tile B, tile A's warp arrives for both
-      // Both warps meet every phase of the barriers in order, used or not: a parity
-      // wait tells a phase only from its neighbours.
+      // Both sides meet every phase of every barrier in order and hand back every slot, and
+      // Q, themselves, used or not: a parity wait tells a phase only from its neighbours, so
+      // nothing may be filled again before both have seen it.
       if (!(ok = kv_wait_warp(&bar.q_full, unit & 1, p.err))) break;
-      // Hands back a slot (or Q) once the MMAs issued so far are done.
-      auto release = [&](uint32_t b) {
-        tc_commit(leader, b);
-        if (twice) tc_commit(leader, b);
-      };
-      if (x == 1 && twice) {
-        for (int k = 0; k < tiles && ok; ++k, ++tk, ++tv)
-          ok = tc_wait(fullK + 8 * (tk & 1), tk >> 1, p.err) && tc_wait(fullV + 8 * (tv & 1), tv >> 1, p.err);
+      if (x == 1 && !w.two) {
+        if (leader) mbar_arrive_at(q_empty);
+        for (int k = 0; k < tiles; ++k, ++tk, ++tv) {
+          if (!(ok = tc_wait(fullK + 8 * (tk & 1), tk >> 1, p.err))) break;
+          if (leader) mbar_arrive_at(emptyK + 8 * (tk & 1));
+          if (!(ok = tc_wait(fullV + 8 * (tv & 1), tv >> 1, p.err))) break;
+          if (leader) mbar_arrive_at(emptyV + 8 * (tv & 1));
+        }
+        __syncwarp();
       } else {
-        if (end == s0) release(q_empty);
+        if (end == s0) tc_commit(leader, q_empty);
         // S(i + 1) = Q K_{i+1}^T, then O += P(i) V_i.
 #pragma unroll 1
         for (int i = s0 - 1; i < end; ++i) {
@@ -382,9 +383,9 @@ __global__ void __launch_bounds__(kTThreads, 1)
             }
             tc_commit(leader, s_full);
             if ((is & 1) || is + 1 == end) {
-              release(emptyK + 8 * (tk & 1));
+              tc_commit(leader, emptyK + 8 * (tk & 1));
               ++tk;
-              if (is + 1 == end) release(q_empty);
+              if (is + 1 == end) tc_commit(leader, q_empty);
             }
             ++n_s;
           }
@@ -399,7 +400,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
               tc_mma_ts(leader, tO, tP + k * 8, vd + k * (2048 >> 4), hiV, idPV, i > s0 || k > 0);
             tc_commit(leader, pv_done + 8 * b);
             if ((i & 1) || i + 1 == end) {
-              release(emptyV + 8 * (tv & 1));
+              tc_commit(leader, emptyV + 8 * (tv & 1));
               ++tv;
             }
             ++n;
@@ -408,8 +409,8 @@ __global__ void __launch_bounds__(kTThreads, 1)
         // Tiles of the run that only the other row tile needs.
         for (int j = (end + 1) >> 1; j < w.last && ok; ++j, ++tk, ++tv) {
           if (!(ok = tc_wait(fullK + 8 * (tk & 1), tk >> 1, p.err) && tc_wait(fullV + 8 * (tv & 1), tv >> 1, p.err))) break;
-          release(emptyK + 8 * (tk & 1));
-          release(emptyV + 8 * (tv & 1));
+          tc_commit(leader, emptyK + 8 * (tk & 1));
+          tc_commit(leader, emptyV + 8 * (tv & 1));
         }
       }
       ++unit;

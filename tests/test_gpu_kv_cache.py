@@ -415,6 +415,24 @@ def test_attention_many_short_requests(ctx, batch, heads, heads_kv, table_pad):
         run(ctx, Batch(new, cached, heads, heads_kv, 16, BF16, seed=hi, table_pad=table_pad if batch < 700 else min(table_pad, 300)))
 
 
+@pytest.mark.parametrize("heads,heads_kv", [(8, 2), (20, 1), (64, 1)])
+@pytest.mark.parametrize("table_pad", [0, 300])
+def test_attention_alternating_row_tiles(ctx, heads, heads_kv, table_pad):
+    """Units of one and of two row tiles in turn, a key tile or two each: the side that
+    has nothing to do in a unit may still be at work on the one before, and no slot may
+    be filled a second time before it has seen the first."""
+    half = 128 // (heads // heads_kv)
+    for seed in range(6):
+        g = torch.Generator().manual_seed(seed)
+        new = [half + 1 + i % half if i % 3 == 0 else 1 + i % half for i in range(240)]
+        cached = torch.randint(0, (1, 100, 200)[seed % 3], (240,), generator=g).tolist()
+        s = Batch(new, cached, heads, heads_kv, 16, BF16, seed=seed, table_pad=table_pad)
+        for _ in range(10):
+            attend(ctx, s)
+        ctx.synchronize()
+        s.check()
+
+
 @pytest.mark.parametrize("new,cached", [([1], [100]), ([1] * 300, [900] * 300), ([1, 1], [9000, 20]), ([20], [400]), ([20], [9000]), ([200], [100])])
 @pytest.mark.parametrize("table_pad", [2, WIDE])
 def test_attention_nan_stays_in_its_row(ctx, new, cached, table_pad):
