@@ -523,7 +523,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
 #pragma unroll
         for (int k = 0; k < 32; ++k) {
           const uint64_t y = fma2(f2(s[2 * k], s[2 * k + 1]), c2, nm2);
-          const uint64_t e = (k & 3) == 3 ? ex2_poly2(y) : f2(ex2(f2lo(y)), ex2(f2hi(y)));
+          const uint64_t e = (k & 3) == 3 ? ex2_poly2_zero(y) : f2(ex2(f2lo(y)), ex2(f2hi(y)));
           sp[k & 3] = add2(sp[k & 3], e);
           pk[k] = kv_pack2<F16>(f2lo(e), f2hi(e));
           // P V of step n - 2, which read this buffer, was issued before the scores of step n.

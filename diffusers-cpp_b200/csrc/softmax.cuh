@@ -82,23 +82,41 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // 2^x of a pair on the FMA / integer pipes, for a share of the softmax exponentials
 // (the MUFU unit alone would limit the softmax: one ex2 per 512 tensor
 // FLOPs is exactly its throughput).  Range reduction x = n + f with
-// n = round(x) (the 1.5 * 2^23 rounding trick), f in [-1/2, 1/2]; 2^f by a
-// degree-3 polynomial fitted here to minimise the maximum relative error on
-// that interval (7.5e-5, far below the bf16 rounding P gets next); 2^n is
-// added to the exponent field.  x is clamped to -126 (masked keys give
-// ~2^-126 instead of 0, which vanishes in bf16 sums of O(1) terms).
-__device__ __forceinline__ uint64_t ex2_poly2(uint64_t x) {
-  x = f2(fmaxf(f2lo(x), -126.0f), fmaxf(f2hi(x), -126.0f));
+// n = round(x) (the 1.5 * 2^23 rounding trick: t holds n in its low bits), f in
+// [-1/2, 1/2]; 2^f by a degree-3 polynomial fitted here to minimise the maximum
+// relative error on that interval (7.5e-5: 1/52 of a half step of bf16, 1/7 to 1/3 of one of f16).
+__device__ __forceinline__ uint64_t ex2_poly2_reduced(uint64_t x, uint64_t& t) {
   const uint64_t magic = f2(12582912.0f, 12582912.0f), neg_magic = f2(-12582912.0f, -12582912.0f);
-  const uint64_t t = add2(x, magic);
+  t = add2(x, magic);
   const uint64_t n = add2(t, neg_magic);
   const uint64_t f = fma2(n, f2(-1.0f, -1.0f), x);
   uint64_t p = fma2(f2(0.0551716648f, 0.0551716648f), f, f2(0.24261114f, 0.24261114f));
   p = fma2(p, f, f2(0.693260968f, 0.693260968f));
-  p = fma2(p, f, f2(0.999928057f, 0.999928057f));
+  return fma2(p, f, f2(0.999928057f, 0.999928057f));
+}
+
+// 2^n is added to the exponent field.  x is clamped to -126 (masked keys give
+// ~2^-126 instead of 0, which vanishes in bf16 sums of O(1) terms).
+__device__ __forceinline__ uint64_t ex2_poly2(uint64_t x) {
+  x = f2(fmaxf(f2lo(x), -126.0f), fmaxf(f2hi(x), -126.0f));
+  uint64_t t;
+  const uint64_t p = ex2_poly2_reduced(x, t);
   const uint32_t lo = static_cast<uint32_t>(p) + ((static_cast<uint32_t>(t) - 0x4B400000u) << 23);
   const uint32_t hi = static_cast<uint32_t>(p >> 32) + ((static_cast<uint32_t>(t >> 32) - 0x4B400000u) << 23);
   return (static_cast<uint64_t>(hi) << 32) | lo;
+}
+
+// The same with a true 0 for -infinity and everything below -126.5: a masked key's
+// value may be as large as the type allows (2^-126 of 3e38 is 3.5).  x is clamped to
+// -127, and 2^n is a factor built in the exponent field, which is 0 for n = -127; one
+// product more a pair.
+__device__ __forceinline__ uint64_t ex2_poly2_zero(uint64_t x) {
+  x = f2(fmaxf(f2lo(x), -127.0f), fmaxf(f2hi(x), -127.0f));
+  uint64_t t;
+  const uint64_t p = ex2_poly2_reduced(x, t);
+  const uint32_t lo = (static_cast<uint32_t>(t) << 23) + 0x3F800000u;  // the trick's own bits leave at the top
+  const uint32_t hi = (static_cast<uint32_t>(t >> 32) << 23) + 0x3F800000u;
+  return mul2(p, (static_cast<uint64_t>(hi) << 32) | lo);
 }
 
 }  // namespace dcpp

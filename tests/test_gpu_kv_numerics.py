@@ -1,0 +1,63 @@
+"""GPU tests of the paged attention's numerics at the edges of its types: values that a
+mask hides, weights far below the largest one, and long caches row by row."""
+import pytest
+import torch
+
+import dcpp_b200
+from kv_util import Batch
+
+pytestmark = pytest.mark.gpu
+BF16, F16 = torch.bfloat16, torch.float16
+WIDE = 9000  # a table this wide makes the attention cut its units into parts
+
+
+def attend(ctx, s, causal=True):
+    cache = dcpp_b200.KVCache(s.k, s.v)
+    ws = torch.full((ctx.kv_attention_workspace(cache, s.heads, s.max_new),), 255, dtype=torch.uint8, device="cuda")
+    ctx.kv_attention(cache, s.q, s.cu_new, s.seq_lens, s.table, s.max_new, ws, s.out, causal=causal)
+    ctx.synchronize()
+
+
+def put(s, b):
+    """Request b's keys and values (s.keys[b], s.values[b]) into its blocks, NaN behind them."""
+    n = s.kv[b]
+    ids = s.table[b, :-(-n // s.block)].long()
+    for src, dst in ((s.keys[b], s.k), (s.values[b], s.v)):
+        pad = torch.full((ids.numel() * s.block - n,) + src.shape[1:], float("nan"), dtype=src.dtype)
+        dst[ids] = torch.cat([src, pad]).unflatten(0, (-1, s.block)).transpose(1, 2).cuda()
+
+
+@pytest.mark.parametrize("new,cached,pad", [(4, 60, 2), (20, 0, 2), (20, 300, 2), (20, 300, WIDE), (150, 0, 2), (150, 1000, WIDE)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_hidden_values_of_any_size_have_no_weight(ctx, new, cached, pad, dtype):
+    """Values that causal order hides from a row, as large as the type allows: the row
+    is what it is without them.  (2^-126 of 3e38 is not small.)"""
+    s = Batch([new], [cached], 8, 2, 16, dtype, table_pad=pad)
+    attend(ctx, s)
+    want = s.out.clone()
+    rows = new // 2
+    s.values[0][cached + rows:] = torch.finfo(dtype).max
+    s.values[0][cached + rows::2] *= -1
+    put(s, 0)
+    attend(ctx, s)
+    assert torch.equal(s.out[:rows], want[:rows])
+
+
+@pytest.mark.parametrize("new,pad", [(1, 2), (20, 2), (20, WIDE), (150, 2)])
+def test_values_of_vanishing_weight_vanish(ctx, new, pad):
+    """Keys 200 below the largest score (e^-200 < 2^-126) with values of 3e38: no trace
+    of them."""
+    s = Batch([new], [400], 8, 2, 16, BF16, table_pad=pad)
+    s.q[..., 0] = 16.0
+    s.keys[0][:, :, 0] = 0.0
+    s.keys[0][5::9, :, 0] = -160.0  # 16 * 160 * 128^-0.5 = 226 lower
+    s.keys[0][:, :, 1:] *= 0.1
+    s.values[0][5::9] = 3e38
+    put(s, 0)
+    attend(ctx, s)
+    big = s.out.clone()
+    s.values[0][5::9] = 0.0
+    put(s, 0)
+    attend(ctx, s)
+    assert torch.equal(s.out, big)
+    s.check()
