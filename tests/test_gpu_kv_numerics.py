@@ -60,3 +60,33 @@ def test_values_of_vanishing_weight_vanish(ctx, new, pad):
     attend(ctx, s)
     assert torch.equal(s.out, big)
     s.check()
+
+
+@pytest.mark.parametrize("new,kv,pad", [(1, 700, 2), (1, 5000, 2), (1, 30000, 2), (4, 30000, WIDE), (20, 700, 2), (20, 3000, 2),
+                                        (20, 30000, WIDE), (300, 900, 2), (300, 30000, 2)])
+@pytest.mark.parametrize("lower", [15.0, 16.5, 18.0])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_weights_far_below_the_largest(ctx, new, kv, pad, lower, dtype):
+    """One key takes nearly all the weight and has the value 0; the others lie `lower`
+    below it and share a value of 1, so what is left of their weights is the output.
+
+    The bound is Batch's and f16's fixed step: numerators are kept 2^13 (up to 16 rows of
+    a group) or 2^6 times larger, relative to a maximum that is the largest score or below
+    it, so each is off by at most 2^-25 2^-13 or 2^-25 2^-6 of the largest weight besides
+    its half step.  Outputs of f16 below 2^-14 (700 e^-18 is 2^-16.5) are themselves
+    rounded to multiples of 2^-24: half of that."""
+    s = Batch([new], [kv - new], 8, 2, 16, dtype, seed=kv, table_pad=pad)
+    s.q.mul_(0.1)
+    s.q[..., 0] = 16.0
+    s.keys[0].mul_(0.05)
+    s.keys[0][:, :, 0] = 0.0
+    s.keys[0][0, :, 0] = lower / (16 * 128 ** -0.5)
+    s.values[0][:] = 1.0
+    s.values[0][0] = 0.0
+    put(s, 0)
+    attend(ctx, s)
+    ref, bound = s.reference(True)
+    if dtype == F16:
+        bound = bound + kv * 2.0 ** (-38 if new * 4 <= 16 else -31) + 2.0 ** -25
+    off = ((s.out[:s.tokens].double() - ref).abs() / bound).max().item()
+    assert off <= 1.0, off
