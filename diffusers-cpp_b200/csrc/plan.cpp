@@ -578,7 +578,7 @@ void StepPlanner::run_ops(std::vector<Op>& ops, cudaGraphExec_t* graph) {
     // Inside a capture the records become graph event nodes (external
     // flag); outside they are ordinary stream records.
     cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-    cuda_check(cudaStreamIsCapturing(s, &cs), "cudaStreamIsCapturing");
+    cuda_check(cudaStreamIsCapturing(ctx_.stream, &cs), "cudaStreamIsCapturing");
     const unsigned flags = cs == cudaStreamCaptureStatusActive ? cudaEventRecordExternal : cudaEventRecordDefault;
     for (size_t i = 0; i < ops.size(); ++i) {
       cudaStream_t os = op_stream(ops[i].stream);
@@ -597,15 +597,23 @@ void StepPlanner::run_ops(std::vector<Op>& ops, cudaGraphExec_t* graph) {
   }
   if (!*graph) {
     cudaGraph_t g = nullptr;
-    cuda_check(cudaStreamBeginCapture(s, cudaStreamCaptureModeThreadLocal), "begin capture");
+    // The legacy default stream cannot be captured (a graph can be launched on it): the ops
+    // are recorded on the context's own stream then.
+    struct OnStream {
+      cudaStream_t &at, was;
+      ~OnStream() { at = was; }
+    } back{ctx_.stream, s};
+    if (s == cudaStreamLegacy) ctx_.stream = ctx_.own_stream;
+    const cudaStream_t rec = ctx_.stream;
+    cuda_check(cudaStreamBeginCapture(rec, cudaStreamCaptureModeThreadLocal), "begin capture");
     try {
       issue();
     } catch (...) {
-      cudaStreamEndCapture(s, &g);
+      cudaStreamEndCapture(rec, &g);
       if (g) cudaGraphDestroy(g);
       throw;
     }
-    cuda_check(cudaStreamEndCapture(s, &g), "end capture");
+    cuda_check(cudaStreamEndCapture(rec, &g), "end capture");
     cudaError_t e = cudaGraphInstantiate(graph, g, 0);
     cudaGraphDestroy(g);
     cuda_check(e, "graph instantiate");
