@@ -13,6 +13,7 @@
 // Rows of one key / value head: the `group` query heads that share it times the
 // tokens of a unit, so that K and V are read once for all of them.
 #include "kv_device.cuh"
+#include "kv_form.cuh"
 #include "kv_sched.cuh"
 
 #include <algorithm>
@@ -58,8 +59,6 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 // among them; their four partial results are joined once per unit.  Measured, 32 heads
 // over 8: 64 requests of 100 to 8000 keys 192 us (6.1 TB/s), 1 of 131k keys 94 us
 // (5.7 TB/s), 1 of 517 keys 6.8 us.
-constexpr int kRRows = 16;
-constexpr int kRKT = 64;
 constexpr int kRStages = 3;
 constexpr int kRHalf = kRKT * 128;          // 8 KB: 64 keys x 64 channels
 constexpr int kRStageBytes = 4 * kRHalf;    // K lo, K hi, V lo, V hi
@@ -69,10 +68,6 @@ constexpr int kRSmem = kRStages * kRStageBytes + kRJoinBytes + 1024;
 // Fewest tiles of a part.  Measured with 2 / 4 / 6, 8 heads over 1: 12k keys 12.1 / 13.5 /
 // 15.6 us, 60k keys 19.0 / 16.9 / 17.8 us.
 constexpr int kRMinTiles = 2;
-// Longest share of a CTA in the direct form.  4 requests of up to 1500 keys, 32 heads over 8:
-// 9.1 us direct, 14.5 us cut; 1 of 12k keys, 8 heads over 1 (24 tiles to a CTA): 25.1 us
-// direct, 12.1 us cut.
-constexpr int kRDirectTiles = 12;
 // Numerators are at most 2^lift (the maximum is never stale): three bits below f16's largest
 // value, for the rounding of maximum x scale (half a step: 2 at 2^25).
 template <bool F16>
@@ -737,31 +732,10 @@ cudaError_t launch_kv_attention(const KvCacheView& c, KvAttnArgs a, const KvAttn
   a.cuts = reinterpret_cast<KvCut*>(ws);
   a.part_ml = reinterpret_cast<float2*>(ws + plan.cut_bytes);
   a.part_o = reinterpret_cast<float*>(ws + plan.cut_bytes + plan.ml_bytes);
-  // Short units (by the table's width, all that the host knows of the lengths) are not
-  // cut at all: a CTA for each, no search for its share and no second kernel.  Measured,
-  // cut / direct: 1 request x 517 keys 12.9 / 6.8 us, 4 ragged prompts of up to
-  // 512 tokens 36.0 / 27.9 us.
+  const KvAttnForm form = kv_attention_form(a, plan);
+  a.direct = form.direct;
   const bool tc = plan.unit_rows == kTcRows;
-  const int64_t longest = (a.max_kv + (tc ? kTcKT : kRKT) - 1) / (tc ? kTcKT : kRKT);
-  const int64_t units = (a.max_new + plan.unit_tokens - 1) / plan.unit_tokens;
-  const int64_t all = units * a.batch * a.heads_kv;
-  // Few units: a cluster of CTAs for each, as large as still fits the GPU at once (clusters
-  // of 8 one to an SM do not fill every SM).
-  int cluster = 1;
-  const int64_t at_once = tc ? plan.grid - plan.grid / 8 : plan.grid;
-  const bool two = tc && std::min<int64_t>(a.max_new, plan.unit_tokens) * a.group > kTcRows / 2;
-  while (cluster < 8 && 2 * cluster * all <= at_once && (two ? 4 * cluster <= longest : cluster < longest)) cluster *= 2;
-  // How long a CTA's share may be.  tcgen05 kernel, in clusters: not much longer than the
-  // cut form's (one of kTcMinTiles or a balanced one); joining units of two row tiles takes
-  // longer.  Measured, cut / clusters: 1 request x 4 tokens x 8 heads a group over 4000 keys
-  // 20.5 / 13.7 us, over 11000 keys 20.5 / 24.4 us; 16 such requests over 4000 keys 26.7 /
-  // 21.5 us, over 7500 keys 34.9 / 32.0 us; 32 tokens over 8000 keys 22.7 / 25.3 us.
-  int64_t most = tc ? kTcDirectTiles : kRDirectTiles;
-  if (tc && cluster > 1)
-    most = std::min<int64_t>(kTcClusterTiles, std::max<int64_t>(kTcMinTiles, all * longest / plan.grid) + (two ? 2 : 4));
-  if (longest <= most * cluster && all <= (1 << 20)) a.direct = static_cast<int32_t>(units);
-  if (!a.direct) cluster = 1;
-  const int ctas = a.direct ? static_cast<int>(all) * cluster : plan.grid;
+  const int ctas = form.ctas, cluster = form.cluster;
   cudaError_t e;
   if (tc)
     e = launch_kv_tc(c, a, ctas, cluster, s);

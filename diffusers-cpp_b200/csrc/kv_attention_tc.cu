@@ -28,6 +28,7 @@
 // requests of 5 tokens over 700 to 4000 keys 20.8 us.
 // TMEM (512 columns): tile X at 128 X: S 0 .. 63, P 64 and 96; O_A 256, O_B 384.
 #include "kv_device.cuh"
+#include "kv_form.cuh"
 #include "kv_sched.cuh"
 
 #include <algorithm>

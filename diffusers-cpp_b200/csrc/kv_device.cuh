@@ -121,11 +121,6 @@ cudaError_t kv_cache_map(CUtensorMap* m, const KvCacheView& c, const void* base,
 cudaError_t kv_query_map(CUtensorMap* m, const KvAttnArgs& a, bool f16, int box_tokens);
 
 // The tensor-core kernel for many query rows (kv_attention_tc.cu).
-constexpr int kTcKT = 128;         // keys of a tile
-constexpr int kTcRows = 256;       // query rows of a unit: two tiles of 128
-constexpr int kTcMinTiles = 4;     // fewest key tiles of a part
-constexpr int kTcDirectTiles = 8;  // longest unit of the direct form
-constexpr int kTcClusterTiles = 16;  // longest share of a CTA in a cluster
 cudaError_t launch_kv_tc(const KvCacheView& c, KvAttnArgs a, int ctas, int cluster, cudaStream_t s);
 
 }  // namespace dcpp
