@@ -482,8 +482,13 @@ __global__ void __launch_bounds__(kStreamWarps * 32, 1)
         turn.load(s_cs);
       }
     }
-    const bool ok = kv_wait_warp(&full[b], (k >> 1) & 1, p.err);
-    if (ok && slot >= 0 && slot < p.n_slots) {
+    if (!kv_wait_warp(&full[b], (k >> 1) & 1, p.err)) {
+      // A barrier whose copy has not landed must not be armed again: no more work, but the
+      // other copy has its own time to land.
+      if (more) kv_wait_warp(&full[b ^ 1], ((k + 1) >> 1) & 1, p.err);
+      return;
+    }
+    if (slot >= 0 && slot < p.n_slots) {
       const StoreDst to(p, t, slot);
       const uint8_t* row = buf + b * (kSliceVecs * 256) + l * 16;
       const int end = min(slice_vecs, n_vec - s * slice_vecs);
