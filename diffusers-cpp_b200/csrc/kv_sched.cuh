@@ -15,29 +15,31 @@
 
 namespace dcpp {
 
-// sum_{i < n} floor((a i + b) / m): the Euclid-like floor-sum recurrence (as in
-// the AtCoder Library's floor_sum).  All values below 2^31.
+// sum_{i < n} floor((a i + b) / m), all values below 2^31.
+//
+// Whole multiples of m in a and b come out as sums of i and of 1.  With a, b < m the terms
+// rise from 0 to T = floor((a (n - 1) + b) / m); counted level by level, term i reaches
+// level j from i = ceil((j m - b) / a) on, so the sum is
+//   sum_{j = 1..T} (n - ceil((j m - b) / a)) = n T - sum_{j < T} floor((m j + m - b + a - 1) / a),
+// the same kind of sum with a and m in each other's place: a few turns, as in Euclid's
+// algorithm.
 static __host__ __device__ __noinline__ int64_t kv_floor_sum(int64_t n, uint32_t m, uint32_t a, uint32_t b) {
-  int64_t ans = 0;
-  uint32_t nn = static_cast<uint32_t>(n);
-  while (nn > 0) {
-    if (a >= m) {
-      ans += static_cast<int64_t>(nn) * (nn - 1) / 2 * (a / m);
-      a %= m;
-    }
-    if (b >= m) {
-      ans += static_cast<int64_t>(nn) * (b / m);
-      b %= m;
-    }
-    const uint32_t top = a * nn + b;  // a < m <= 128, nn <= 2^24
-    if (top < m) break;
-    nn = top / m;
-    b = top % m;
-    const uint32_t t = m;
+  int64_t sum = 0, sign = 1;
+  while (n > 0) {
+    const uint32_t qa = a / m, qb = b / m;
+    sum += sign * (n * (n - 1) / 2 * qa + n * qb);
+    a -= qa * m;
+    b -= qb * m;
+    const int64_t levels = (a * static_cast<uint32_t>(n - 1) + b) / m;  // a < 128, n <= 2^24
+    sum += sign * n * levels;
+    b = m - b + a - 1;
+    const uint32_t was = m;
     m = a;
-    a = t;
+    a = was;
+    n = levels;  // 0 if a was
+    sign = -sign;
   }
-  return ans;
+  return sum;
 }
 
 // One sequence's share of the work.
