@@ -255,7 +255,15 @@ typedef struct dcpp_kv_cache {
  * (free blocks, max_blocks, max_tokens) or whose lengths or counters make no
  * sense is refused as a whole: cu_new 0, slots -1, seq_lens = cached, counters
  * and table unchanged; dcpp_synchronize reports DCPP_ERR_OOM or
- * DCPP_ERR_INVALID_ARG.  Outputs must not overlap the other arrays. */
+ * DCPP_ERR_INVALID_ARG.  Outputs must not overlap the other arrays.
+ *
+ * The plan knows no owners: a block has one place, in the ring or in one row of
+ * the table.  Rows that name the same blocks can be attended to, but a block
+ * given back by two of them is in the ring twice, and two later requests write
+ * it, without a report.  Block ids are not part of what refuses a step: one
+ * outside the cache is reported (DCPP_ERR_INVALID_ARG) and moves on as it is,
+ * from the ring into the table (the tokens of its block get slot -1) or from a
+ * finished request's row into the ring, whose counters advance as ever. */
 dcpp_status dcpp_kv_plan(dcpp_ctx* ctx, const dcpp_kv_cache* cache, int64_t batch, const int32_t* d_cached,
                          const int32_t* d_new, int32_t* d_free_blocks, const int64_t* d_free_in, int64_t* d_free_out,
                          int32_t* d_block_table, int64_t max_blocks, int32_t* d_seq_lens, int32_t* d_cu_new,
