@@ -142,3 +142,34 @@ class Batch:
         off = torch.where(tiny, 0, off)
         assert off.numel() == 0 or off.max().item() <= 1.0, f"error {off.max().item():.3f} of its bound at {off.argmax().item()}"
         assert (self.out[self.tokens:] == 7.0).all(), "rows behind the last request were written"
+
+
+def row_norm_check(q, k, v, got, scale, u, seen=None, lost=None):
+    """The largest error of a row's 128 outputs together, as a share of what it may be:
+    q [rows, D], k, v [keys, D] and got [rows, D] in float64, seen [rows, keys] (None:
+    all).  v has to be of independent normal values.  `lost`: keys that the reference
+    leaves out (a planted mistake).
+
+    A bound per value has to add up every key's rounding as if all had one sign.  Their
+    sum over a row's channels does not: numerator j is off by a share t_j of its own, which
+    depends on q and k alone, so the error sum_j t_j p_j v_j is a normal vector whose
+    channels have a variance of at most t^2 sum p^2, and its norm exceeds 1.5 sqrt(128)
+    of that once in 10^13 (chi-square of 128 degrees).  t: a half step u of the type, 2^-13
+    for the exponential and 2 mag 128 2^-23 for a 128-term f32 score (Batch.reference).
+    The f32 sums take n / 16 + 32 steps at most, each off by 2^-22 of a partial sum, itself
+    normal and below 8 sqrt(sum p^2).  The sum of the numerators and the output's own
+    rounding move the whole row: u + 2^-13 + 2 mag 128 2^-23 + (n / 16 + 32) 2^-24 of it."""
+    s = q @ k.T * scale
+    mag = ((q.abs() @ k.abs().T).amax(-1, keepdim=True) * scale)
+    if seen is not None:
+        s = s.masked_fill(~seen, -math.inf)
+    if lost is not None:
+        s[:, lost] = -math.inf
+    p = torch.softmax(s, -1)
+    o = p @ v
+    n = k.shape[0]
+    spread = p.square().sum(-1, keepdim=True).sqrt() * D ** 0.5
+    shift = 2 ** -13 + 2 * mag * 128 * 2 ** -23
+    steps = n / 16 + 32
+    bound = spread * (1.5 * (u + shift) + steps * 2 ** -19) + o.norm(dim=-1, keepdim=True) * (u + shift + steps * 2 ** -24)
+    return ((got - o).norm(dim=-1, keepdim=True) / bound).max().item()
