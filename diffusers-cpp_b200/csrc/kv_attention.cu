@@ -57,8 +57,8 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 // The four consumer warps each own 16 keys of every tile: scores, running maximum,
 // numerators and all 128 output columns of their keys, so the loop has no barrier
 // among them; their four partial results are joined once per unit.  Measured, 32 heads
-// over 8: 64 requests of 100 to 8000 keys 192 us (6.1 TB/s), 1 of 131k keys 94 us
-// (5.7 TB/s), 1 of 517 keys 6.8 us.
+// over 8: 64 requests of 100 to 8000 keys 186 us (6.3 TB/s), 1 of 131k keys 90 us
+// (6.0 TB/s), 1 of 517 keys 6.8 us.
 constexpr int kRStages = 3;
 constexpr int kRHalf = kRKT * 128;          // 8 KB: 64 keys x 64 channels
 constexpr int kRStageBytes = 4 * kRHalf;    // K lo, K hi, V lo, V hi

@@ -21,11 +21,12 @@
 // V stays as the cache holds it, keys x channels: the P V product takes it as an
 // operand whose rows run along the channels (MN-major), so no transposed copy of the
 // cache is kept.
-// Measured, 32 heads over 8: two prompts of 8k tokens 935 to 1015 us (1040 to 1130
+// Measured in a graph, 32 heads over 8: two prompts of 8k tokens 940 to 1030 us (1020 to 1120
 // TFLOP/s; the products alone take some 775 us, the softmax alone 870 us), 512 tokens
-// over 32k keys 250 us (1080 TFLOP/s), 4 prompts of 301 to 512 tokens 22 to 28 us
+// over 32k keys 255 us (1070 TFLOP/s), 4 prompts of 301 to 512 tokens 20 to 26 us
 // (launch, first loads and last stores of two units for most CTAs); 16 heads over 2, 16
-// requests of 5 tokens over 700 to 4000 keys 20.8 us.
+// requests of 5 tokens over 700 to 4000 keys 19 to 21 us.  Called back to back for a tenth of
+// a second the power cap lowers the clock: 1050 us (1000 TFLOP/s) and 301 us (904 TFLOP/s).
 // TMEM (512 columns): tile X at 128 X: S 0 .. 63, P 64 and 96; O_A 256, O_B 384.
 #include "kv_device.cuh"
 #include "kv_form.cuh"

@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_plan_kernel(const __grid_c
 // shared by all heads of the token: computed once into shared memory by the
 // first 64 threads, as fractions of a turn in 64-bit fixed point (the product with
 // the position wraps, which drops whole turns; what is left is off by position *
-// 2^-56 turns, so a far position is as good as a near one), then cos and sin of
+// 2^-55 turns, so a far position is as good as a near one), then cos and sin of
 // [-1/2, 1/2] turn.  Sums and the rotation are f32 (two values an instruction),
 // rounded once to the cache's type.
 constexpr int kStoreThreads = 128;

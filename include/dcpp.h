@@ -304,10 +304,19 @@ dcpp_status dcpp_kv_store(dcpp_ctx* ctx, const dcpp_kv_cache* cache, int64_t tok
  *   workspace  dcpp_kv_attention_workspace bytes, 16-byte aligned; need not be
  *           cleared, keeps nothing between calls; calls that may run at the same
  *           time (other streams, graphs replayed side by side) need their own
+ * The table's width (max_blocks) is all that the host knows of the lengths: where
+ * it says that requests are short, a batch of few rows takes about two thirds of
+ * the time (one request over 517 keys 6.7 us, 11.4 us with a table of 32k keys).
  * Block table entries beyond a request's tokens, and what its last block holds
  * behind them, are never used.  A NaN in a row of q, or in a key that the row
  * attends to, makes the row NaN; a value that causal order hides still meets the
  * weight 0 (0 x inf is NaN), so a request's cached values have to be finite.
+ * Numerics: scores, maxima and sums in f32 (scores below 2^24 in size).  Each
+ * exp(s_j - m) is rounded to the cache's type for its product with v_j, half a
+ * step (2^-8 or 2^-11 of it) besides 2^-13 of its own, and in f16 2^-31 of the
+ * row's largest; the sum that divides them is not rounded.  Against f32 weights
+ * the error of the outputs is up to 1.4 times as large (bf16, relative to their
+ * size: 0.0023 where the output's rounding alone makes 0.0017).
  * Lengths or block ids out of range leave the request's rows undefined and are
  * reported by dcpp_synchronize (DCPP_ERR_INVALID_ARG).  Up to 128 query heads per
  * key / value head, max_blocks * block_size below 2^31 - 4096. */
