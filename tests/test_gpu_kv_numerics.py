@@ -90,3 +90,28 @@ def test_weights_far_below_the_largest(ctx, new, kv, pad, lower, dtype):
         bound = bound + kv * 2.0 ** (-38 if new * 4 <= 16 else -31) + 2.0 ** -25
     off = ((s.out[:s.tokens].double() - ref).abs() / bound).max().item()
     assert off <= 1.0, off
+
+
+@pytest.mark.parametrize("new,pad", [(1, 2), (4, WIDE), (20, 2), (20, WIDE), (150, 2)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_scores_of_many_millions(ctx, new, pad, dtype):
+    """Scores up to 2^23, thousands apart: each row is the value of its largest key.  The
+    numerator (2^lift times the rounding of maximum x scale) and the output are rounded once
+    each, the f32 division by the sum is off by 2^-23."""
+    s = Batch([new], [700], 8, 2, 16, dtype, table_pad=pad)
+    s.q.zero_()
+    s.q[..., 0] = 8192.0
+    g = torch.Generator().manual_seed(new)
+    k = (11000.0 - 64 * torch.randperm(s.kv[0], generator=g)[:, None].expand(-1, 2)).to(dtype)  # 8192 * 11000 * 128^-0.5 < 2^23
+    s.keys[0].zero_()
+    s.keys[0][:, :, 0] = k
+    put(s, 0)
+    attend(ctx, s)
+    best = torch.stack([k[:s.kv[0] - new + i + 1, 0].float().argmax() for i in range(new)])
+    size = k[best, 0].float()
+    clear = torch.tensor([(k[:s.kv[0] - new + i + 1, 0].float() == size[i]).sum() == 1 for i in range(new)])
+    assert clear.sum() > new // 2 or clear.all()
+    u = torch.finfo(dtype).eps / 2
+    want = s.values[0][best].double().repeat_interleave(4, 1)  # [new, 8, 128]
+    got = s.out[:new].double().cpu()
+    assert ((got - want).abs() <= (2 * u + u * u + 2 ** -22) * want.abs() + torch.finfo(dtype).tiny)[clear].all()
